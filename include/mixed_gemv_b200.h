@@ -315,6 +315,101 @@ typedef struct mgv_launch_info {
 } mgv_launch_info;
 mgv_status mgv_gemv_launch_info(const mgv_gemv_args *args, mgv_launch_info *info);
 
+/* ---- the 8-bit activation path: prompts and larger batches on int8 layers ----
+ *
+ * The GEMV above keeps activations in 16 bits and serves up to 16 rows.  A prompt, or a batch of
+ * any size, goes through an int8 layer with int8 activations instead: a norm or a row
+ * quantisation gives every row (token) int8 values and one fp32 scale, and an int8 matrix product
+ * with 32-bit integer sums applies the scale of the row and of the output feature in its
+ * epilogue.  No counterpart in the reference, which stops at one row and 16-bit activations.
+ *
+ * int8 rows [rows][ld] are row-major, scales fp32 [rows], value = q * scale.  Quantisation is
+ * symmetric: scale = max|v| / 127, q = v * 127 / max|v| rounded to the nearest integer, ties to
+ * even; -128 never occurs.  A row of zeros has scale 0; a row with an infinity or a NaN has scale
+ * NaN and q = 0, so whatever is computed from it is NaN, and other rows are not touched by it.
+ * Elements of a q row from K to its leading dimension are left as they were.
+ *
+ * All calls are asynchronous, allocate nothing, keep no state between calls and may be captured.
+ * M = 0 (no rows) is a valid call that launches nothing.  MGV_FLAG_PDL works as in the GEMV: the
+ * kernel may start while its predecessor on the stream drains, and touches only norm weights,
+ * layer weights, their scales and bias before that predecessor has completed. */
+
+typedef enum mgv_dtype { MGV_DTYPE_F16 = 0, MGV_DTYPE_BF16 = 1, MGV_DTYPE_F32 = 2 } mgv_dtype;
+
+/* x [M][ldx] (dtype: F16 or BF16) -> q int8 [M][ldq], scale fp32 [M].  Any K >= 1 and any leading
+ * dimensions >= K; x at its element's alignment, scale 4-byte aligned.  Rows whose addresses are
+ * multiples of 16 bytes (q: 8) are read and written in vectors.  flags: MGV_FLAG_PDL. */
+mgv_status mgv_quantize_rows(void *q_i8_dev, void *scale_f32_dev, const void *x_dev, int dtype, int64_t M, int32_t K,
+                             int64_t ldq, int64_t ldx, int flags, mgv_stream_t s);
+
+/* The way back: out[m][k] = round(q[m][k] * scale[m]) in dtype (F16 or BF16), [M][ldo]. */
+mgv_status mgv_dequantize_rows(void *out_dev, const void *q_i8_dev, const void *scale_f32_dev, int dtype, int64_t M,
+                               int32_t K, int64_t ldo, int64_t ldq, int flags, mgv_stream_t s);
+
+/* Root-mean-square norm with the residual's addition in front and the quantisation behind it:
+ *   h = x + residual rounded to dtype (h = x without a residual); residual_out = h
+ *   y = h / sqrt(mean_k(h^2) + eps) * weight, in fp32;  q, scale = the quantised rows of y
+ * The norm is taken of the rounded h: what a later layer reads back from residual_out. */
+typedef struct mgv_rmsnorm_args {
+  int32_t struct_size;
+  int32_t dtype;          /* F16 or BF16: x, residual, weight, residual_out                  */
+  int32_t flags;          /* MGV_FLAG_PDL                                                     */
+  int32_t K;              /* row length, >= 1                                                 */
+  int64_t M;              /* rows, >= 0                                                       */
+  const void *x;          /* [M][ldx]                                                         */
+  const void *residual;   /* [M][ldr] or NULL                                                 */
+  const void *weight;     /* [K]                                                              */
+  void *residual_out;     /* [M][ldro]; given exactly when residual is; may be x or residual  */
+                          /* itself (same address and leading dimension), not overlap otherwise */
+  void *q;                /* int8 [M][ldq]                                                    */
+  void *scale;            /* fp32 [M]                                                         */
+  int64_t ldx, ldr, ldro, ldq;
+  float eps;              /* >= 0, finite                                                     */
+} mgv_rmsnorm_args;
+
+/* Fills *args with defaults (struct_size, eps = 1e-5). */
+void mgv_rmsnorm_args_init(mgv_rmsnorm_args *args);
+mgv_status mgv_rmsnorm_quantize(const mgv_rmsnorm_args *args, mgv_stream_t s);
+
+/* int8 matrix product with a scale for each row (token) and each output feature:
+ *   v[m][n] = x_scale[m] * weight_scale[n] * sum_k x[m][k] * weights[n][k] + bias[n]
+ *   out[m][n] = round(act(v[m][n]))
+ * The sum is exact (32-bit integers), so results do not depend on how the work is divided; the
+ * epilogue computes in fp32 and rounds once.  weights are NOT preprocessed: the int8 matrix as
+ * mgv_preprocess_weights takes it with MGV_LAYOUT_COLUMN_MAJOR, K contiguous for each feature.
+ * A layer that also decodes through mgv_gemv keeps both forms (the GEMV's interleave follows the
+ * reference and is not one the tensor cores' 8-bit operands can be copied from).  flags:
+ * MGV_FLAG_ACT_RELU or MGV_FLAG_ACT_SILU (not both); MGV_FLAG_GATED_SILU as in the GEMV: rows 2i
+ * and 2i+1 of weights, scales and bias are gate and up, out has N/2 features; MGV_FLAG_PDL. */
+typedef struct mgv_gemm_i8_args {
+  int32_t struct_size;
+  int32_t N;                /* output features, >= 1; even with MGV_FLAG_GATED_SILU            */
+  int32_t K;                /* reduction length, 1..131071 (the sum must fit 32 bits)          */
+  int32_t out_dtype;        /* F16 or BF16: out and bias                                       */
+  int32_t scale_dtype;      /* F16, BF16 or F32: weight_scale                                  */
+  int32_t flags;            /* MGV_FLAG_*                                                      */
+  int64_t M;                /* rows of x and out, 0..2^31-1                                    */
+  const void *x;            /* int8 [M][ldx], 16-byte aligned                                  */
+  const void *weights;      /* int8 [N][ldw], 16-byte aligned                                  */
+  const void *x_scale;      /* fp32 [M]                                                        */
+  const void *weight_scale; /* [N]                                                             */
+  const void *bias;         /* [N] in out_dtype, or NULL                                       */
+  void *out;                /* [M][ldd] in out_dtype                                           */
+  int64_t ldx, ldw;         /* bytes between rows, multiples of 16, >= K                       */
+  int64_t ldd;              /* elements between rows of out                                    */
+  int32_t hints;            /* MGV_GEMM_HINT_* (0: the library chooses)                        */
+  int32_t reserved;         /* 0                                                               */
+} mgv_gemm_i8_args;
+
+/* Fills *args with defaults (struct_size; everything else 0). */
+void mgv_gemm_i8_args_init(mgv_gemm_i8_args *args);
+mgv_status mgv_gemm_i8(const mgv_gemm_i8_args *args, mgv_stream_t s);
+/* The same in two steps, as mgv_gemv_plan_*: buffers are captured and must stay where they are. */
+typedef struct mgv_gemm_i8_plan mgv_gemm_i8_plan;
+mgv_status mgv_gemm_i8_plan_create(const mgv_gemm_i8_args *args, mgv_gemm_i8_plan **plan);
+mgv_status mgv_gemm_i8_plan_run(const mgv_gemm_i8_plan *plan, mgv_stream_t s);
+void mgv_gemm_i8_plan_destroy(mgv_gemm_i8_plan *plan);
+
 /* ---- a resident layer: the flow of main(), mixed_gemv_test.cu:245-283, behind one handle ----
  * These are the only entry points that allocate device memory. */
 

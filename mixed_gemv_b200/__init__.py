@@ -5,8 +5,8 @@ The product is ``libmixed_gemv_b200.so`` (hand-written CUDA behind the C ABI dec
 mirrors the reference's interface (``api``), seeded synthetic inputs (``synth``) and the
 multi-GPU sharding helpers (``sharded``).  There is no CPU or PyTorch fallback.
 """
-from .enums import LayoutType, QuantType, Status, Variant, WeightOnlyQuantOp, has_zero, is_finegrained
+from .enums import DType, LayoutType, QuantType, Status, Variant, WeightOnlyQuantOp, has_zero, is_finegrained
 from ._lib import MgvError
 
-__all__ = ["LayoutType", "QuantType", "Status", "Variant", "WeightOnlyQuantOp", "has_zero",
+__all__ = ["DType", "LayoutType", "QuantType", "Status", "Variant", "WeightOnlyQuantOp", "has_zero",
            "is_finegrained", "MgvError"]

@@ -45,6 +45,27 @@ class LaunchInfo(C.Structure):
                                            "tile_rows", "k_slice", "split_tiles")]
 
 
+class RmsNormArgs(C.Structure):
+    """mgv_rmsnorm_args"""
+    _fields_ = [
+        ("struct_size", C.c_int32), ("dtype", C.c_int32), ("flags", C.c_int32), ("K", C.c_int32), ("M", C.c_int64),
+        ("x", C.c_void_p), ("residual", C.c_void_p), ("weight", C.c_void_p), ("residual_out", C.c_void_p),
+        ("q", C.c_void_p), ("scale", C.c_void_p),
+        ("ldx", C.c_int64), ("ldr", C.c_int64), ("ldro", C.c_int64), ("ldq", C.c_int64), ("eps", C.c_float),
+    ]
+
+
+class GemmI8Args(C.Structure):
+    """mgv_gemm_i8_args"""
+    _fields_ = [
+        ("struct_size", C.c_int32), ("N", C.c_int32), ("K", C.c_int32), ("out_dtype", C.c_int32),
+        ("scale_dtype", C.c_int32), ("flags", C.c_int32), ("M", C.c_int64),
+        ("x", C.c_void_p), ("weights", C.c_void_p), ("x_scale", C.c_void_p), ("weight_scale", C.c_void_p),
+        ("bias", C.c_void_p), ("out", C.c_void_p),
+        ("ldx", C.c_int64), ("ldw", C.c_int64), ("ldd", C.c_int64), ("hints", C.c_int32), ("reserved", C.c_int32),
+    ]
+
+
 FLAG_OUT_F32_PARTIAL = 1
 FLAG_ACT_RELU = 2
 FLAG_ACT_SILU = 4
@@ -67,6 +88,8 @@ EXPORTS = [
     "mgv_window_destroy", "mgv_wait_arrivals", "mgv_reduce_partials", "mgv_wait_reduce_partials",
     "mgv_gemv_launch_info", "mgv_linear_create", "mgv_linear_forward_host", "mgv_linear_forward",
     "mgv_linear_weights", "mgv_linear_destroy",
+    "mgv_quantize_rows", "mgv_dequantize_rows", "mgv_rmsnorm_args_init", "mgv_rmsnorm_quantize",
+    "mgv_gemm_i8_args_init", "mgv_gemm_i8", "mgv_gemm_i8_plan_create", "mgv_gemm_i8_plan_run", "mgv_gemm_i8_plan_destroy",
 ]
 
 _lib = None
@@ -115,10 +138,24 @@ def load() -> C.CDLL:
     lib.mgv_window_destroy.argtypes = [vp]
     lib.mgv_wait_arrivals.argtypes = [vp, vp, C.c_uint32, C.c_uint32, vp]
     lib.mgv_reduce_partials.argtypes = [vp, sz, i32, i32, i32, C.c_longlong, vp, C.c_float, i32, vp, C.c_longlong, vp]
+    i64 = C.c_int64
+    lib.mgv_quantize_rows.argtypes = [vp, vp, vp, i32, i64, C.c_int32, i64, i64, i32, vp]
+    lib.mgv_dequantize_rows.argtypes = [vp, vp, vp, i32, i64, C.c_int32, i64, i64, i32, vp]
+    lib.mgv_rmsnorm_args_init.argtypes = [C.POINTER(RmsNormArgs)]
+    lib.mgv_rmsnorm_args_init.restype = None
+    lib.mgv_rmsnorm_quantize.argtypes = [C.POINTER(RmsNormArgs), vp]
+    lib.mgv_gemm_i8_args_init.argtypes = [C.POINTER(GemmI8Args)]
+    lib.mgv_gemm_i8_args_init.restype = None
+    lib.mgv_gemm_i8.argtypes = [C.POINTER(GemmI8Args), vp]
+    lib.mgv_gemm_i8_plan_create.argtypes = [C.POINTER(GemmI8Args), C.POINTER(vp)]
+    lib.mgv_gemm_i8_plan_run.argtypes = [vp, vp]
+    lib.mgv_gemm_i8_plan_destroy.argtypes = [vp]
+    lib.mgv_gemm_i8_plan_destroy.restype = None
     for name in EXPORTS:
         fn = getattr(lib, name)
         if name not in ("mgv_status_string", "mgv_last_error", "mgv_version", "mgv_gemv_args_init",
-                        "mgv_linear_weights", "mgv_linear_destroy", "mgv_gemv_plan_destroy"):
+                        "mgv_linear_weights", "mgv_linear_destroy", "mgv_gemv_plan_destroy", "mgv_rmsnorm_args_init",
+                        "mgv_gemm_i8_args_init", "mgv_gemm_i8_plan_destroy"):
             fn.restype = i32
     _lib = lib
     return lib

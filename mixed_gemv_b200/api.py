@@ -9,6 +9,13 @@ calls ``exit(-1)`` these raise :class:`MgvError` carrying the library's status.
     MixedGemvWeightPreprocessor.run    utils/preprocess.h:480-522
     GemvAdaptor / Arguments            gemv/device/gemv_adaptor.h:59-262
     device_gemv                        mixed_gemv_test.cu:124-165
+
+The 8-bit activation path (no counterpart there) follows the adaptor's manner, arguments in a dataclass,
+initialize() once and run() as often as wanted:
+
+    RmsNormQuantizer                   norm with the residual's addition, int8 rows and their scales out
+    RowQuantizer / RowDequantizer      16-bit rows to int8 rows with scales, and back
+    GemmI8Adaptor                      int8 matrix product with scales for each row and output feature
 """
 from __future__ import annotations
 
@@ -19,8 +26,8 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from ._lib import GemvArgs, LaunchInfo, MgvError, check
-from .enums import LayoutType, QuantType, Variant, WeightOnlyQuantOp
+from ._lib import GemmI8Args, GemvArgs, LaunchInfo, MgvError, RmsNormArgs, check
+from .enums import DType, LayoutType, QuantType, Variant, WeightOnlyQuantOp
 
 
 def _stream_ptr(stream) -> int:
@@ -317,3 +324,205 @@ class Linear:
             self.close()
         except Exception:
             pass
+
+
+# ---- the 8-bit activation path ------------------------------------------------------------------
+
+_DTYPES = {torch.float16: DType.F16, torch.bfloat16: DType.BF16, torch.float32: DType.F32}
+
+
+def _rows(t: torch.Tensor, name: str, shape, dtypes, device) -> int:
+    """Address of a [rows, columns] tensor whose rows may be apart (stride(0)) but are dense."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise MgvError(1, f"{name} must be a CUDA tensor (this library has no CPU path)")
+    if device is not None and t.device != device:
+        raise MgvError(1, f"{name} is on {t.device}, the call on {device}")
+    if t.dtype not in dtypes:
+        raise MgvError(2, f"{name} must be one of {[str(d) for d in dtypes]}, not {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise MgvError(1, f"{name} must have the shape {tuple(shape)}, not {tuple(t.shape)}")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise MgvError(1, f"{name} must be dense along its last dimension")
+    return t.data_ptr()
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Elements between rows; of a single row, where any stride is meant alike, a valid one."""
+    return max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0)
+
+
+def _ld16(t: torch.Tensor) -> int:
+    """_ld where rows start at multiples of 16 bytes: of a single int8 row that is no demand on its length."""
+    return -(-_ld(t) // 16) * 16 if t.shape[0] <= 1 else _ld(t)
+
+
+def _two_dims(t: torch.Tensor, name: str):
+    if not isinstance(t, torch.Tensor) or t.dim() != 2:
+        raise MgvError(1, f"{name} must be a tensor of two dimensions (rows, columns)")
+    return int(t.shape[0]), int(t.shape[1])
+
+
+class _RowOperator:
+    """initialize() checks the arguments and lays out the call once, run() only launches, calling
+    the object does both.  Buffers are captured and must stay where they are."""
+
+    def __init__(self):
+        self._call = None
+        self._keep = None
+
+    def initialize(self, args, stream=None) -> None:
+        self._call = None
+        self._device, self._call = self._prepare(_lib.load(), args)
+        self._keep = args
+
+    def run(self, stream=None) -> None:
+        if self._call is None:
+            raise MgvError(1, f"{type(self).__name__}.run() before initialize()")
+        if torch.cuda.current_device() != self._device:
+            raise MgvError(1, f"{type(self).__name__} was initialized for device {self._device}, "
+                              f"current is {torch.cuda.current_device()}")
+        status = self._call(_stream_ptr(stream))
+        if status:
+            check(status)
+
+    def __call__(self, args, stream=None) -> None:
+        self.initialize(args, stream)
+        self.run(stream)
+
+
+@dataclass
+class RowQuantizeArguments:
+    """q, scale = the rows of x in int8 (mgv_quantize_rows)."""
+    x: torch.Tensor                      # fp16 / bf16 [M, K]
+    q: torch.Tensor                      # int8 [M, K]
+    scale: torch.Tensor                  # fp32 [M]
+    flags: int = 0
+
+
+class RowQuantizer(_RowOperator):
+    def _prepare(self, lib, a: RowQuantizeArguments):
+        M, K = _two_dims(a.x, "x")
+        x = _rows(a.x, "x", (M, K), (torch.float16, torch.bfloat16), None)
+        q = _rows(a.q, "q", (M, K), (torch.int8,), a.x.device)
+        scale = _rows(a.scale, "scale", (M,), (torch.float32,), a.x.device)
+        fixed = (q, scale, x, int(_DTYPES[a.x.dtype]), M, K, _ld(a.q), _ld(a.x), int(a.flags))
+        return a.x.device.index, lambda s: lib.mgv_quantize_rows(*fixed, s)
+
+
+@dataclass
+class RowDequantizeArguments:
+    """out = q * scale of its row, rounded to out's type (mgv_dequantize_rows)."""
+    q: torch.Tensor                      # int8 [M, K]
+    scale: torch.Tensor                  # fp32 [M]
+    out: torch.Tensor                    # fp16 / bf16 [M, K]
+    flags: int = 0
+
+
+class RowDequantizer(_RowOperator):
+    def _prepare(self, lib, a: RowDequantizeArguments):
+        M, K = _two_dims(a.q, "q")
+        q = _rows(a.q, "q", (M, K), (torch.int8,), None)
+        scale = _rows(a.scale, "scale", (M,), (torch.float32,), a.q.device)
+        out = _rows(a.out, "out", (M, K), (torch.float16, torch.bfloat16), a.q.device)
+        fixed = (out, q, scale, int(_DTYPES[a.out.dtype]), M, K, _ld(a.out), _ld(a.q), int(a.flags))
+        return a.q.device.index, lambda s: lib.mgv_dequantize_rows(*fixed, s)
+
+
+@dataclass
+class RmsNormQuantizeArguments:
+    """h = x + residual; q, scale = the rows of h / rms(h) * weight in int8; residual_out = h
+    (mgv_rmsnorm_quantize).  Without a residual h = x and nothing but q and scale is written."""
+    x: torch.Tensor                      # fp16 / bf16 [M, K]
+    weight: torch.Tensor                 # [K], x's type
+    q: torch.Tensor                      # int8 [M, K]
+    scale: torch.Tensor                  # fp32 [M]
+    residual: Optional[torch.Tensor] = None      # [M, K], x's type
+    residual_out: Optional[torch.Tensor] = None  # [M, K]; may be residual or x itself
+    eps: float = 1e-5
+    flags: int = 0
+
+
+class RmsNormQuantizer(_RowOperator):
+    def _prepare(self, lib, a: RmsNormQuantizeArguments):
+        M, K = _two_dims(a.x, "x")
+        dev, same = a.x.device, (a.x.dtype,)
+        c = RmsNormArgs()
+        lib.mgv_rmsnorm_args_init(C.byref(c))
+        c.x = _rows(a.x, "x", (M, K), (torch.float16, torch.bfloat16), None)
+        c.weight = _rows(a.weight, "weight", (K,), same, dev)
+        c.q = _rows(a.q, "q", (M, K), (torch.int8,), dev)
+        c.scale = _rows(a.scale, "scale", (M,), (torch.float32,), dev)
+        if (a.residual is None) != (a.residual_out is None):
+            raise MgvError(1, "residual and residual_out are given together or not at all")
+        if a.residual is not None:
+            c.residual = _rows(a.residual, "residual", (M, K), same, dev)
+            c.residual_out = _rows(a.residual_out, "residual_out", (M, K), same, dev)
+            c.ldr, c.ldro = _ld(a.residual), _ld(a.residual_out)
+        c.dtype, c.flags, c.M, c.K = int(_DTYPES[a.x.dtype]), int(a.flags), M, K
+        c.ldx, c.ldq, c.eps = _ld(a.x), _ld(a.q), float(a.eps)
+        ref = C.byref(c)
+        return dev.index, lambda s: lib.mgv_rmsnorm_quantize(ref, s)
+
+
+@dataclass
+class GemmI8Arguments:
+    """out = act(x weights^T * x_scale * weight_scale + bias) (mgv_gemm_i8).  weights are the int8 matrix of
+    the layer as it is before preprocessing, one row per output feature; rows of x and weights start at multiples of
+    16 bytes.  With FLAG_GATED_SILU rows 2i and 2i + 1 are gate and up, and out has N / 2 columns."""
+    x: torch.Tensor                      # int8 [M, K]
+    x_scale: torch.Tensor                # fp32 [M]
+    weights: torch.Tensor                # int8 [N, K]
+    weight_scale: torch.Tensor           # fp16 / bf16 / fp32 [N]
+    out: torch.Tensor                    # fp16 / bf16 [M, N]
+    bias: Optional[torch.Tensor] = None  # [N], out's type
+    flags: int = 0
+    hints: int = 0                       # _lib.GEMM_HINT_*: forces a code path (tests, tuning)
+
+
+class GemmI8Adaptor(_RowOperator):
+    """initialize() checks the arguments and plans the launch (mgv_gemm_i8_plan_create), run() only
+    launches (mgv_gemm_i8_plan_run), calling the object does both."""
+
+    def __init__(self):
+        super().__init__()
+        self._plan = None
+
+    def _drop_plan(self):
+        if getattr(self, "_plan", None):
+            _lib.load().mgv_gemm_i8_plan_destroy(self._plan)
+            self._plan = None
+
+    def __del__(self):
+        try:
+            self._drop_plan()
+        except Exception:
+            pass
+
+    @staticmethod
+    def _to_c(lib, a: GemmI8Arguments) -> GemmI8Args:
+        (M, K), (N, _) = _two_dims(a.x, "x"), _two_dims(a.weights, "weights")
+        gated = bool(int(a.flags) & _lib.FLAG_GATED_SILU)
+        dev = a.x.device
+        c = GemmI8Args()
+        lib.mgv_gemm_i8_args_init(C.byref(c))
+        c.x = _rows(a.x, "x", (M, K), (torch.int8,), None)
+        c.weights = _rows(a.weights, "weights", (N, K), (torch.int8,), dev)
+        c.x_scale = _rows(a.x_scale, "x_scale", (M,), (torch.float32,), dev)
+        c.weight_scale = _rows(a.weight_scale, "weight_scale", (N,), tuple(_DTYPES), dev)
+        c.out = _rows(a.out, "out", (M, N // 2 if gated else N), (torch.float16, torch.bfloat16), dev)
+        if a.bias is not None:
+            c.bias = _rows(a.bias, "bias", (N,), (a.out.dtype,), dev)
+        c.M, c.N, c.K, c.flags, c.hints = M, N, K, int(a.flags), int(a.hints)
+        c.out_dtype, c.scale_dtype = int(_DTYPES[a.out.dtype]), int(_DTYPES[a.weight_scale.dtype])
+        c.ldx, c.ldw, c.ldd = _ld16(a.x), _ld16(a.weights), _ld(a.out)
+        return c
+
+    def _prepare(self, lib, a: GemmI8Arguments):
+        c = self._to_c(lib, a)
+        self._drop_plan()
+        if torch.cuda.current_device() != a.x.device.index:
+            raise MgvError(1, f"the tensors are on device {a.x.device.index}, current is {torch.cuda.current_device()}")
+        plan = C.c_void_p()
+        check(lib.mgv_gemm_i8_plan_create(C.byref(c), C.byref(plan)))
+        self._plan = plan
+        return a.x.device.index, lambda s: lib.mgv_gemm_i8_plan_run(plan, s)

@@ -50,3 +50,10 @@ class Variant(IntEnum):
     AUTO = 0
     SIMT = 1
     MMA = 2
+
+
+class DType(IntEnum):
+    """mgv_dtype of include/mixed_gemv_b200.h"""
+    F16 = 0
+    BF16 = 1
+    F32 = 2
