@@ -37,6 +37,7 @@ def is_stale() -> bool:
         return True
     t = os.path.getmtime(LIB_PATH)
     deps = sources() + [os.path.join(CSRC, "mgv_common.cuh"), os.path.join(CSRC, "mgv_gemv_parts.cuh"),
+                        os.path.join(CSRC, "mgv_gemm_parts.cuh"),
                         os.path.join(INCLUDE, "mixed_gemv_b200.h")]
     return any(os.path.getmtime(d) > t for d in deps)
 

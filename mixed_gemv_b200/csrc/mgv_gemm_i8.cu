@@ -1,80 +1,159 @@
-// int8 matrix product with a scale for each row and each output feature: entry points, plan and kernel.
-#include <cuda_bf16.h>
-
+// int8 matrix product with a scale for each row and each output feature: entry points, plan and kernels.
+#include <algorithm>
+#include <mutex>
 #include <new>
 
-#include "mgv_common.cuh"
+#include "mgv_gemm_parts.cuh"
 
 namespace mgv {
 
-struct GemmI8Params {
-  const int8_t *x, *w;
-  const float *x_scale;
-  const void *w_scale, *bias;
-  void *out;
-  int64_t ldx, ldw, ldd;
-  int M, N, K, out_dtype, scale_dtype, flags;
-};
+// One tile -- 128 output features x p.bt activation rows -- per cluster of p.split blocks, each with
+// its share of K.  The weights are the matrix instruction's 128-row operand and the activations its
+// column operand, whose width goes from 16 up: one token costs a sixteen-column tile, not 128 rows.
+// Weights and activations reach a ring of shared-memory slots by tiled bulk copies, one thread issues
+// the matrix instructions, accumulators are 32-bit integers in tensor memory: lane = feature, column =
+// row of the activations.  With split > 1 every block leaves its sums in shared memory and block r
+// adds and finishes the r-th part of the columns out of all of them; integer sums, so the result
+// does not depend on the split.
+template <int ACT, bool BF16>
+__global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_block_kernel(const __grid_constant__ GemmI8Params p) {
+  extern __shared__ uint8_t dynamic[];
+  __shared__ alignas(8) uint64_t full[kGemmMaxStages], empty[kGemmMaxStages], done;
+  __shared__ uint32_t tmem_base;
+  __shared__ int failed;
+  __shared__ alignas(16) float x_scale[256];
+  const uint32_t ring = (smem_u32(dynamic) + 1023) & ~1023u;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t rank = p.split > 1 ? cluster_rank() : 0;
+  const uint32_t tile = blockIdx.x / uint32_t(p.split);
+  const int n0 = int(tile % uint32_t(p.n_tiles)) * kGemmRows, m0 = int(tile / uint32_t(p.n_tiles)) * p.bt;
+  const int slices = (p.K + kGemmK - 1) / kGemmK;
+  const int first = int(int64_t(slices) * rank / p.split), count = int(int64_t(slices) * (rank + 1) / p.split) - first;
+  const uint32_t slot_bytes = kGemmABytes + p.bt * kGemmK;
 
-__device__ __forceinline__ float load_as_float(const void *p, int64_t i, int dtype) {
-  if (dtype == MGV_DTYPE_F16) return __half2float(static_cast<const __half *>(p)[i]);
-  if (dtype == MGV_DTYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
-  return static_cast<const float *>(p)[i];
-}
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < p.stages; ++i) bar_init(smem_u32(&full[i]), 1), bar_init(smem_u32(&empty[i]), 1);
+    bar_init(smem_u32(&done), 1);
+    failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(p.tmem_cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = tmem_base;
+  // only now: a dependent kernel that starts on this SM may hold tensor memory while it waits for this one to end
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-__device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
+  if (warp == 0 && lane == 0) {
+    // weights of the first ring fill before the wait for the previous kernel, its output (x) after it
+    const int ahead = min(count, p.stages);
+    for (int i = 0; i < ahead; ++i) {
+      bar_expect(smem_u32(&full[i]), slot_bytes);
+      box_load(ring + i * slot_bytes, &p.w_map, (first + i) * kGemmK, n0, smem_u32(&full[i]));
+    }
+    asm volatile("griddepcontrol.wait;\n\tfence.proxy.async.global;" ::: "memory");
+    for (int i = 0; i < ahead; ++i) box_load(ring + i * slot_bytes + kGemmABytes, &p.x_map, (first + i) * kGemmK, m0, smem_u32(&full[i]));
+    int slot = 0, issued = ahead;
+    uint32_t phase = 0;
+    for (int i = ahead; i < count; ++i) {
+      if (!bar_wait(smem_u32(&empty[slot]), phase, p.err)) break;
+      const uint32_t bar = smem_u32(&full[slot]), dst = ring + slot * slot_bytes;
+      bar_expect(bar, slot_bytes);
+      box_load(dst, &p.w_map, (first + i) * kGemmK, n0, bar);
+      box_load(dst + kGemmABytes, &p.x_map, (first + i) * kGemmK, m0, bar);
+      ++issued;
+      if (++slot == p.stages) slot = 0, phase ^= 1;
+    }
+    // no copy may be in flight when the block ends: the last ones are waited for, whoever else gave up
+    for (int i = max(0, issued - p.stages); i < issued; ++i)
+      if (!bar_wait(smem_u32(&full[i % p.stages]), (i / p.stages) & 1, p.err)) break;
+  } else if (warp == 1 && lane == 0) {
+    int slot = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int i = 0; i < count && ok; ++i) {
+      ok = bar_wait(smem_u32(&full[slot]), phase, p.err);
+      if (!ok) break;
+      tmem_fence_after();
+      const uint64_t a = operand_desc(ring + slot * slot_bytes), b = operand_desc(ring + slot * slot_bytes + kGemmABytes);
+#pragma unroll
+      for (int k = 0; k < kGemmK / 32; ++k) {  // 32 bytes of K per instruction: two 16-byte steps of the descriptors
+        const uint32_t add = i + k > 0;
+        asm volatile(
+            "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, q;\n\t}" ::"r"(tmem),
+            "l"(a + 2 * k), "l"(b + 2 * k), "r"(p.idesc), "r"(add)
+            : "memory");
+      }
+      asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&empty[slot])) : "memory");
+      if (++slot == p.stages) slot = 0, phase ^= 1;
+    }
+    if (!ok) *static_cast<volatile int *>(&failed) = 1;
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&done)) : "memory");
+  }
 
-constexpr int kSimpleTile = 64, kSimpleK = 16;  // 64 x 64 outputs, 16 words (64 values) of K at a time
-
-// 64 x 64 outputs per block through shared memory, four-way int8 dot products.
-__global__ void __launch_bounds__(256) gemm_i8_simple_kernel(GemmI8Params p) {
-  __shared__ int xs[kSimpleK][kSimpleTile + 1], ws[kSimpleK][kSimpleTile + 1];
-  const int n0 = blockIdx.x * kSimpleTile, tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  for (int64_t m0 = int64_t(blockIdx.y) * kSimpleTile; m0 < p.M; m0 += int64_t(gridDim.y) * kSimpleTile) {
-    int acc[4][4] = {};
-    for (int k0 = 0; k0 < p.K; k0 += 4 * kSimpleK) {
-      for (int i = threadIdx.x; i < kSimpleTile * kSimpleK; i += 256) {
-        const int row = i / kSimpleK, kw = i % kSimpleK, k = k0 + 4 * kw;
-        int xv = 0, wv = 0;
-        for (int b = 0; b < 4; ++b) {
-          if (k + b >= p.K) break;
-          if (m0 + row < p.M) xv |= int(uint8_t(p.x[(m0 + row) * p.ldx + k + b])) << (8 * b);
-          if (n0 + row < p.N) wv |= int(uint8_t(p.w[int64_t(n0 + row) * p.ldw + k + b])) << (8 * b);
+  // tensor memory: a warp reads the 32 lanes of its number modulo 4
+  const int quarter = warp % 4, row = quarter * 32 + lane;
+  const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
+  bool good = true;
+  Feature f = {};
+  if (warp >= 2) {
+    f = load_feature<BF16>(p, n0 + row);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (int i = threadIdx.x - 64; i < p.bt; i += 128) x_scale[i] = m0 + i < p.M ? p.x_scale[m0 + i] : 0.0f;
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    good = bar_wait(smem_u32(&done), 0, p.err) && !*static_cast<volatile int *>(&failed);
+    good = __all_sync(~0u, good);
+    tmem_fence_after();
+    const int columns = min(p.bt, p.M - m0);
+    if (p.split == 1) {
+      if (good)
+        for (int c = 0; c < columns; c += 16) {
+          int v[16];
+          tmem_load16(lanes + c, v);
+          tmem_wait_load();
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) finish_pair<ACT, BF16>(p, f, m0 + c + i, v[i], v[i + 1], x_scale[c + i], x_scale[c + i + 1]);
         }
-        xs[kw][row] = xv;
-        ws[kw][row] = wv;
-      }
-      __syncthreads();
-      for (int kw = 0; kw < kSimpleK; ++kw)
-        for (int i = 0; i < 4; ++i)
-          for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(xs[kw][ty * 4 + i], ws[kw][tx * 4 + j], acc[i][j]);
-      __syncthreads();
-    }
-    for (int i = 0; i < 4; ++i) {
-      const int64_t m = m0 + ty * 4 + i;
-      if (m >= p.M) continue;
-      const float sx = p.x_scale[m];
-      float v[4];
-      for (int j = 0; j < 4; ++j) {
-        const int n = n0 + tx * 4 + j;
-        v[j] = 0.0f;
-        if (n >= p.N) continue;
-        v[j] = float(acc[i][j]) * (sx * load_as_float(p.w_scale, n, p.scale_dtype));
-        if (p.bias) v[j] += load_as_float(p.bias, n, p.out_dtype);
-        if (p.flags & MGV_FLAG_ACT_RELU) v[j] = v[j] < 0.0f ? 0.0f : v[j];
-        if (p.flags & MGV_FLAG_ACT_SILU) v[j] = silu(v[j]);
-      }
-      const bool gated = p.flags & MGV_FLAG_GATED_SILU;
-      for (int j = 0; j < 4; j += gated ? 2 : 1) {
-        const int n = n0 + tx * 4 + j;
-        if (n >= p.N) continue;
-        const float y = gated ? silu(v[j]) * v[j + 1] : v[j];
-        const int64_t at = m * p.ldd + (gated ? n / 2 : n);
-        if (p.out_dtype == MGV_DTYPE_F16) static_cast<__half *>(p.out)[at] = __float2half_rn(y);
-        else static_cast<__nv_bfloat16 *>(p.out)[at] = __float2bfloat16_rn(y);
+    } else {
+      // every copy has landed and every matrix instruction has read its slot: the ring's memory is free
+      for (int c = 0; c < columns; c += 16) {
+        int v[16];
+        tmem_load16(lanes + c, v);
+        tmem_wait_load();
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(ring + ((c + i) * kGemmRows + row) * 4), "r"(v[i]) : "memory");
       }
     }
+    tmem_fence_before();
+  }
+  if (p.split > 1) {
+    cluster_sync();
+    if (warp >= 2 && good) {
+      const int share = p.bt / p.split, c0 = int(rank) * share, c1 = min(c0 + share, p.M - m0);
+      for (int c = c0; c < c1; c += 2) {
+        int a0 = 0, a1 = 0;
+        for (int b = 0; b < p.split; ++b) {
+          const uint32_t at = in_block(ring, b) + (c * kGemmRows + row) * 4;
+          a0 += load_cluster(at);
+          a1 += load_cluster(at + kGemmRows * 4);
+        }
+        finish_pair<ACT, BF16>(p, f, m0 + c, a0, a1, x_scale[c], x_scale[c + 1]);
+      }
+    }
+    cluster_sync();  // no block ends while another may still read its sums
+  } else {
+    __syncwarp();
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tmem_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
   }
 }
 
@@ -116,32 +195,140 @@ using namespace mgv;
 
 struct mgv_gemm_i8_plan {
   GemmI8Params p;
-  int device = 0;
+  int device = 0, grid = 0, smem = 0, act = 0, bf16 = 0, flags = 0;
 };
 
-static mgv_status prepare(const mgv_gemm_i8_args *a, mgv_gemm_i8_plan &pl) {
-  const mgv_status st = check_args(a);
-  if (st != MGV_STATUS_OK) return st;
-  MGV_CUDA_TRY(cudaGetDevice(&pl.device));
-  pl.p = {static_cast<const int8_t *>(a->x), static_cast<const int8_t *>(a->weights), static_cast<const float *>(a->x_scale),
-          a->weight_scale, a->bias, a->out, a->ldx, a->ldw, a->ldd, int(a->M), a->N, a->K, a->out_dtype, a->scale_dtype, a->flags};
+// A dense int8 matrix [rows][ld] as boxes of 128 bytes of K x box_rows rows, in the 128-byte swizzle
+// that the matrix instruction reads; what lies beyond K or the last row arrives as zeros.
+static mgv_status encode_rows(CUtensorMap *map, const void *ptr, int64_t rows, int K, int64_t ld, int box_rows) {
+  using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                              const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static Encode encode = nullptr;
+  static std::mutex mu;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (!encode) {
+      void *fn = nullptr;
+      cudaDriverEntryPointQueryResult q;
+      MGV_CUDA_TRY(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q));
+      if (q != cudaDriverEntryPointSuccess || !fn) return fail(MGV_STATUS_CUDA_ERROR, "gemm_i8: the driver has no cuTensorMapEncodeTiled");
+      encode = reinterpret_cast<Encode>(fn);
+    }
+  }
+  const cuuint64_t dims[2] = {cuuint64_t(K), cuuint64_t(rows)}, strides[1] = {cuuint64_t(ld)};
+  const cuuint32_t box[2] = {kGemmK, cuuint32_t(box_rows)}, elem[2] = {1, 1};
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(ptr), dims, strides, box, elem,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MGV_STATUS_CUDA_ERROR, "gemm_i8: cuTensorMapEncodeTiled failed (%d)", int(r));
   return MGV_STATUS_OK;
+}
+
+static mgv_status prepare(const mgv_gemm_i8_args *a, mgv_gemm_i8_plan &pl) {
+  mgv_status st = check_args(a);
+  if (st != MGV_STATUS_OK) return st;
+  GemmI8Params &p = pl.p;
+  p = GemmI8Params{};
+  pl.flags = a->flags;
+  MGV_CUDA_TRY(cudaGetDevice(&pl.device));
+  if (a->M == 0) return MGV_STATUS_OK;
+  int sms = 0, most = 0;
+  MGV_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, pl.device));
+  MGV_CUDA_TRY(cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, pl.device));
+  p.x_scale = static_cast<const float *>(a->x_scale);
+  p.w_scale = a->weight_scale; p.bias = a->bias; p.out = a->out; p.ldd = a->ldd;
+  p.M = int(a->M); p.N = a->N; p.K = a->K; p.scale_dtype = a->scale_dtype;
+  p.wide = reinterpret_cast<uintptr_t>(a->out) % 4 == 0 && a->ldd % 2 == 0;
+  p.err = device_error_word();
+  if (!p.err) return fail(MGV_STATUS_CUDA_ERROR, "gemm_i8: no device error word");
+  pl.act = a->flags & MGV_FLAG_ACT_RELU ? kActRelu : a->flags & MGV_FLAG_ACT_SILU ? kActSilu : a->flags & MGV_FLAG_GATED_SILU ? kActGated : kActNone;
+  pl.bf16 = a->out_dtype == MGV_DTYPE_BF16;
+
+  // columns of the matrix instruction: 16, or a multiple of 32 up to 256
+  p.bt = a->M <= 16 ? 16 : int(std::min<int64_t>(256, (a->M + 31) / 32 * 32));
+  if (const int want = (a->hints >> 8) & 31) p.bt = want == 1 ? 16 : std::min(256, (want + 1) / 2 * 32);
+  p.n_tiles = (p.N + kGemmRows - 1) / kGemmRows;
+  const int64_t tiles = p.n_tiles * ((a->M + p.bt - 1) / p.bt);
+  const int slices = (p.K + kGemmK - 1) / kGemmK;
+  p.split = 1;
+  while (p.split < 8 && 2 * p.split <= slices && tiles * p.split < sms * 7 / 8) p.split *= 2;
+  if (const int want = a->hints & 7) p.split = std::min(1 << (want - 1), 8);
+  while (p.split > slices) p.split /= 2;
+  const int64_t grid = tiles * p.split;
+  if (grid > 0x7fffffff) return fail(MGV_STATUS_UNSUPPORTED, "gemm_i8: too many tiles (M=%lld N=%d)", (long long)a->M, a->N);
+  pl.grid = int(grid);
+  p.tmem_cols = 32;
+  while (int(p.tmem_cols) < p.bt) p.tmem_cols *= 2;
+  const int slot = kGemmABytes + p.bt * kGemmK, room = most - 4096;  // static shared memory and alignment
+  const int share = (slices + p.split - 1) / p.split;
+  p.stages = std::min(std::min(share, kGemmMaxStages), (grid > sms ? room / 2 : room) / slot);
+  p.stages = std::max(p.stages, std::min(2, share));
+  // the sums of a split tile need bt x 128 words; and blocks that fit an SM by their shared memory must fit
+  // it by their tensor memory too (512 columns), or one would wait in its allocation for another to end
+  int smem = p.stages * slot;
+  if (p.split > 1) smem = std::max(smem, p.bt * kGemmRows * 4);
+  smem = std::max(smem, int(int64_t(most) * p.tmem_cols / 512));
+  pl.smem = std::min(smem + 1024, room + 1024);
+  // fields of the descriptor: 32-bit integer sums (2 at bit 4), signed operands (1 at bits 7 and 10), N / 8, M / 16
+  p.idesc = 2u << 4 | 1u << 7 | 1u << 10 | uint32_t(p.bt / 8) << 17 | uint32_t(kGemmRows / 16) << 24;
+  if ((st = encode_rows(&p.w_map, a->weights, a->N, a->K, a->ldw, kGemmRows)) != MGV_STATUS_OK) return st;
+  return encode_rows(&p.x_map, a->x, a->M, a->K, a->ldx, p.bt);
+}
+
+template <auto KERN>
+static mgv_status launch_kernel(const mgv_gemm_i8_plan &pl, cudaStream_t s) {
+  static bool configured[64];
+  static std::mutex mu;
+  if (pl.device < 0 || pl.device >= 64) return fail(MGV_STATUS_UNSUPPORTED, "gemm_i8: device index %d beyond 63", pl.device);
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (!configured[pl.device]) {
+      int optin = 0;
+      cudaFuncAttributes fa;
+      MGV_CUDA_TRY(cudaDeviceGetAttribute(&optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, pl.device));
+      MGV_CUDA_TRY(cudaFuncGetAttributes(&fa, KERN));
+      MGV_CUDA_TRY(cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, optin - int(fa.sharedSizeBytes)));
+      configured[pl.device] = true;
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(pl.grid);
+  cfg.blockDim = dim3(kGemmThreads);
+  cfg.dynamicSmemBytes = pl.smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attrs[2];
+  int n = 0;
+  if (pl.p.split > 1) {
+    attrs[n].id = cudaLaunchAttributeClusterDimension;
+    attrs[n].val.clusterDim.x = unsigned(pl.p.split);
+    attrs[n].val.clusterDim.y = attrs[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (pl.flags & MGV_FLAG_PDL) {
+    attrs[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attrs;
+  cfg.numAttrs = n;
+  MGV_CUDA_TRY(cudaLaunchKernelEx(&cfg, KERN, pl.p));
+  return MGV_STATUS_OK;
+}
+
+template <int ACT>
+static mgv_status launch_act(const mgv_gemm_i8_plan &pl, cudaStream_t s) {
+  return pl.bf16 ? launch_kernel<gemm_i8_block_kernel<ACT, true>>(pl, s) : launch_kernel<gemm_i8_block_kernel<ACT, false>>(pl, s);
 }
 
 static mgv_status launch(const mgv_gemm_i8_plan &pl, cudaStream_t s) {
   if (pl.p.M == 0) return MGV_STATUS_OK;
-  cudaLaunchConfig_t cfg = {};
-  const int64_t mt = (int64_t(pl.p.M) + kSimpleTile - 1) / kSimpleTile;
-  cfg.gridDim = dim3((unsigned(pl.p.N) + kSimpleTile - 1) / kSimpleTile, unsigned(mt < 65535 ? mt : 65535));
-  cfg.blockDim = dim3(256);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = (pl.p.flags & MGV_FLAG_PDL) ? 1 : 0;
-  MGV_CUDA_TRY(cudaLaunchKernelEx(&cfg, gemm_i8_simple_kernel, pl.p));
-  return MGV_STATUS_OK;
+  switch (pl.act) {
+    case kActRelu: return launch_act<kActRelu>(pl, s);
+    case kActSilu: return launch_act<kActSilu>(pl, s);
+    case kActGated: return launch_act<kActGated>(pl, s);
+    default: return launch_act<kActNone>(pl, s);
+  }
 }
 
 extern "C" void mgv_gemm_i8_args_init(mgv_gemm_i8_args *a) {
