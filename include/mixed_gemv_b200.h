@@ -383,12 +383,12 @@ mgv_status mgv_rmsnorm_quantize(const mgv_rmsnorm_args *args, mgv_stream_t s);
  * and 2i+1 of weights, scales and bias are gate and up, out has N/2 features; MGV_FLAG_PDL. */
 typedef struct mgv_gemm_i8_args {
   int32_t struct_size;
-  int32_t N;                /* output features, >= 1; even with MGV_FLAG_GATED_SILU            */
+  int32_t N;                /* output features, 1..2^30; even with MGV_FLAG_GATED_SILU         */
   int32_t K;                /* reduction length, 1..131071 (the sum must fit 32 bits)          */
   int32_t out_dtype;        /* F16 or BF16: out and bias                                       */
   int32_t scale_dtype;      /* F16, BF16 or F32: weight_scale                                  */
   int32_t flags;            /* MGV_FLAG_*                                                      */
-  int64_t M;                /* rows of x and out, 0..2^31-1                                    */
+  int64_t M;                /* rows of x and out, 0..2^30                                      */
   const void *x;            /* int8 [M][ldx], 16-byte aligned                                  */
   const void *weights;      /* int8 [N][ldw], 16-byte aligned                                  */
   const void *x_scale;      /* fp32 [M]                                                        */
@@ -400,6 +400,15 @@ typedef struct mgv_gemm_i8_args {
   int32_t hints;            /* MGV_GEMM_HINT_* (0: the library chooses)                        */
   int32_t reserved;         /* 0                                                               */
 } mgv_gemm_i8_args;
+
+/* Plan hints (mgv_gemm_i8_args.hints).  Every combination computes the same bits through another
+ * kernel or tiling; they exist so that tests and tuning runs can reach each path on any shape.
+ * Bits 0..2: blocks that share a tile's K range, as 1 + log2 (0: the library chooses).  Bits 8..12:
+ * rows of x in a tile, in units of 16 (rounded up to what the kernel takes; 0: the library chooses). */
+enum {
+  MGV_GEMM_HINT_BLOCK = 8,  /* the kernel of single blocks (small batches)                        */
+  MGV_GEMM_HINT_PAIR = 16   /* the kernel of block pairs (prompts)                                */
+};
 
 /* Fills *args with defaults (struct_size; everything else 0). */
 void mgv_gemm_i8_args_init(mgv_gemm_i8_args *args);

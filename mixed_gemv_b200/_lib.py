@@ -78,6 +78,18 @@ HINT_ITEM_128, HINT_ITEM_256 = 4, 8
 HINT_KERNEL_GENERAL, HINT_KERNEL_STAGED, HINT_KERNEL_XREG = 16, 32, 48
 HINT_ONE_LAUNCH = 64
 
+# mgv_gemm_i8_args.hints
+GEMM_HINT_BLOCK, GEMM_HINT_PAIR = 8, 16
+
+
+def gemm_hint_split(blocks: int) -> int:
+    return blocks.bit_length()
+
+
+def gemm_hint_rows(rows: int) -> int:
+    return (rows // 16) << 8
+
+
 # every symbol include/mixed_gemv_b200.h declares
 EXPORTS = [
     "mgv_status_string", "mgv_last_error", "mgv_version", "mgv_pack_int4", "mgv_unpack_int4",

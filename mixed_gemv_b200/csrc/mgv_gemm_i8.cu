@@ -114,6 +114,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_block_kernel(const __
       if (good)
         for (int c = 0; c < columns; c += 16) {
           int v[16];
+          __syncwarp();
           tmem_load16(lanes + c, v);
           tmem_wait_load();
 #pragma unroll
@@ -159,8 +160,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_block_kernel(const __
 
 static mgv_status check_args(const mgv_gemm_i8_args *a) {
   if (!a || a->struct_size != int32_t(sizeof(*a))) return fail(MGV_STATUS_INVALID_ARGUMENT, "gemm_i8: args null or of another version");
-  if (a->M < 0 || a->M > 0x7fffffff) return fail(MGV_STATUS_INVALID_ARGUMENT, "gemm_i8: M=%lld outside 0..2^31-1", (long long)a->M);
-  if (a->N < 1) return fail(MGV_STATUS_INVALID_ARGUMENT, "gemm_i8: N=%d must be at least 1", a->N);
+  if (a->M < 0 || a->M > (1 << 30)) return fail(MGV_STATUS_INVALID_ARGUMENT, "gemm_i8: M=%lld outside 0..2^30", (long long)a->M);
+  if (a->N < 1 || a->N > (1 << 30)) return fail(MGV_STATUS_INVALID_ARGUMENT, "gemm_i8: N=%d outside 1..2^30", a->N);
   if (a->K < 1 || a->K > 131071) return fail(MGV_STATUS_INVALID_ARGUMENT, "gemm_i8: K=%d outside 1..131071", a->K);
   if (a->out_dtype != MGV_DTYPE_F16 && a->out_dtype != MGV_DTYPE_BF16)
     return fail(MGV_STATUS_UNSUPPORTED, "gemm_i8: out_dtype %d is neither F16 nor BF16", a->out_dtype);
@@ -193,10 +194,8 @@ static mgv_status check_args(const mgv_gemm_i8_args *a) {
 
 using namespace mgv;
 
-struct mgv_gemm_i8_plan {
-  GemmI8Params p;
-  int device = 0, grid = 0, smem = 0, act = 0, bf16 = 0, flags = 0;
-};
+struct mgv_gemm_i8_plan : GemmI8Plan {};
+
 
 // A dense int8 matrix [rows][ld] as boxes of 128 bytes of K x box_rows rows, in the 128-byte swizzle
 // that the matrix instruction reads; what lies beyond K or the last row arrives as zeros.
@@ -225,6 +224,58 @@ static mgv_status encode_rows(CUtensorMap *map, const void *ptr, int64_t rows, i
   return MGV_STATUS_OK;
 }
 
+// Instruction descriptor: 32-bit integer sums (2 at bit 4), signed operands (1 at bits 7 and 10),
+// columns / 8 at bit 17, rows / 16 at bit 24.
+static uint32_t instruction(int rows, int columns) { return 2u << 4 | 1u << 7 | 1u << 10 | uint32_t(columns / 8) << 17 | uint32_t(rows / 16) << 24; }
+
+static mgv_status plan_block(GemmI8Plan &pl, int64_t M, int bt, int split, int sms, int most) {
+  GemmI8Params &p = pl.p;
+  // columns of the matrix instruction: 16, or a multiple of 32 up to 256
+  p.bt = bt ? bt : M <= 16 ? 16 : int(std::min<int64_t>(256, (M + 31) / 32 * 32));
+  p.n_tiles = (p.N + kGemmRows - 1) / kGemmRows;
+  const int64_t tiles = p.n_tiles * ((M + p.bt - 1) / p.bt);
+  const int slices = (p.K + kGemmK - 1) / kGemmK;
+  p.split = 1;
+  while (p.split < 8 && 2 * p.split <= slices && tiles * p.split < sms * 7 / 8) p.split *= 2;
+  if (split) p.split = std::min(1 << (split - 1), 8);
+  while (p.split > slices) p.split /= 2;
+  const int64_t grid = tiles * p.split;
+  if (grid > 0x7fffffff) return fail(MGV_STATUS_UNSUPPORTED, "gemm_i8: too many tiles (M=%lld N=%d)", (long long)M, p.N);
+  pl.grid = int(grid);
+  pl.cluster = p.split;
+  p.tmem_cols = 32;
+  while (int(p.tmem_cols) < p.bt) p.tmem_cols *= 2;
+  const int slot = kGemmABytes + p.bt * kGemmK, room = most - 4096;  // static shared memory and alignment
+  const int share = (slices + p.split - 1) / p.split;
+  p.stages = std::min(std::min(share, kGemmMaxStages), (grid > sms ? room / 2 : room) / slot);
+  p.stages = std::max(p.stages, std::min(2, share));
+  // the sums of a split tile need bt x 128 words; and blocks that fit an SM by their shared memory must fit
+  // it by their tensor memory too (512 columns), or one would wait in its allocation for another to end
+  int smem = p.stages * slot;
+  if (p.split > 1) smem = std::max(smem, p.bt * kGemmRows * 4);
+  smem = std::max(smem, int(int64_t(most) * p.tmem_cols / 512));
+  pl.smem = std::min(smem + 1024, room + 1024);
+  p.idesc = instruction(kGemmRows, p.bt);
+  return MGV_STATUS_OK;
+}
+
+static void plan_pair(GemmI8Plan &pl, int64_t M, int bt, int sms, int most) {
+  GemmI8Params &p = pl.p;
+  p.bt = bt ? bt : int(std::min<int64_t>(256, (M + 31) / 32 * 32));
+  p.n_tiles = (p.N + 2 * kGemmRows - 1) / (2 * kGemmRows);
+  p.m_tiles = int((M + p.bt - 1) / p.bt);
+  p.split = 1;
+  const int64_t tiles = int64_t(p.n_tiles) * p.m_tiles;
+  pl.grid = int(2 * std::min<int64_t>(tiles, sms / 2));
+  pl.cluster = 2;
+  p.tmem_cols = 64;  // two accumulators
+  while (int(p.tmem_cols) < 2 * p.bt) p.tmem_cols *= 2;
+  const int slot = kGemmABytes + p.bt / 2 * kGemmK, room = most - 4096;
+  p.stages = std::min(kGemmMaxStages, room / slot);
+  pl.smem = room + 1024;  // one block per SM: it may hold all of the tensor memory
+  p.idesc = instruction(2 * kGemmRows, p.bt);
+}
+
 static mgv_status prepare(const mgv_gemm_i8_args *a, mgv_gemm_i8_plan &pl) {
   mgv_status st = check_args(a);
   if (st != MGV_STATUS_OK) return st;
@@ -245,84 +296,22 @@ static mgv_status prepare(const mgv_gemm_i8_args *a, mgv_gemm_i8_plan &pl) {
   pl.act = a->flags & MGV_FLAG_ACT_RELU ? kActRelu : a->flags & MGV_FLAG_ACT_SILU ? kActSilu : a->flags & MGV_FLAG_GATED_SILU ? kActGated : kActNone;
   pl.bf16 = a->out_dtype == MGV_DTYPE_BF16;
 
-  // columns of the matrix instruction: 16, or a multiple of 32 up to 256
-  p.bt = a->M <= 16 ? 16 : int(std::min<int64_t>(256, (a->M + 31) / 32 * 32));
-  if (const int want = (a->hints >> 8) & 31) p.bt = want == 1 ? 16 : std::min(256, (want + 1) / 2 * 32);
-  p.n_tiles = (p.N + kGemmRows - 1) / kGemmRows;
-  const int64_t tiles = p.n_tiles * ((a->M + p.bt - 1) / p.bt);
-  const int slices = (p.K + kGemmK - 1) / kGemmK;
-  p.split = 1;
-  while (p.split < 8 && 2 * p.split <= slices && tiles * p.split < sms * 7 / 8) p.split *= 2;
-  if (const int want = a->hints & 7) p.split = std::min(1 << (want - 1), 8);
-  while (p.split > slices) p.split /= 2;
-  const int64_t grid = tiles * p.split;
-  if (grid > 0x7fffffff) return fail(MGV_STATUS_UNSUPPORTED, "gemm_i8: too many tiles (M=%lld N=%d)", (long long)a->M, a->N);
-  pl.grid = int(grid);
-  p.tmem_cols = 32;
-  while (int(p.tmem_cols) < p.bt) p.tmem_cols *= 2;
-  const int slot = kGemmABytes + p.bt * kGemmK, room = most - 4096;  // static shared memory and alignment
-  const int share = (slices + p.split - 1) / p.split;
-  p.stages = std::min(std::min(share, kGemmMaxStages), (grid > sms ? room / 2 : room) / slot);
-  p.stages = std::max(p.stages, std::min(2, share));
-  // the sums of a split tile need bt x 128 words; and blocks that fit an SM by their shared memory must fit
-  // it by their tensor memory too (512 columns), or one would wait in its allocation for another to end
-  int smem = p.stages * slot;
-  if (p.split > 1) smem = std::max(smem, p.bt * kGemmRows * 4);
-  smem = std::max(smem, int(int64_t(most) * p.tmem_cols / 512));
-  pl.smem = std::min(smem + 1024, room + 1024);
-  // fields of the descriptor: 32-bit integer sums (2 at bit 4), signed operands (1 at bits 7 and 10), N / 8, M / 16
-  p.idesc = 2u << 4 | 1u << 7 | 1u << 10 | uint32_t(p.bt / 8) << 17 | uint32_t(kGemmRows / 16) << 24;
+  const int want = (a->hints >> 8) & 31;
+  pl.pair = a->hints & MGV_GEMM_HINT_PAIR || (!(a->hints & MGV_GEMM_HINT_BLOCK) && a->M > 256);
+  if (pl.pair) plan_pair(pl, a->M, want ? std::min(256, (want + 1) / 2 * 32) : 0, sms, most);
+  else if ((st = plan_block(pl, a->M, want == 1 ? 16 : std::min(256, (want + 1) / 2 * 32), a->hints & 7, sms, most)) != MGV_STATUS_OK) return st;
   if ((st = encode_rows(&p.w_map, a->weights, a->N, a->K, a->ldw, kGemmRows)) != MGV_STATUS_OK) return st;
-  return encode_rows(&p.x_map, a->x, a->M, a->K, a->ldx, p.bt);
-}
-
-template <auto KERN>
-static mgv_status launch_kernel(const mgv_gemm_i8_plan &pl, cudaStream_t s) {
-  static bool configured[64];
-  static std::mutex mu;
-  if (pl.device < 0 || pl.device >= 64) return fail(MGV_STATUS_UNSUPPORTED, "gemm_i8: device index %d beyond 63", pl.device);
-  {
-    std::lock_guard<std::mutex> lock(mu);
-    if (!configured[pl.device]) {
-      int optin = 0;
-      cudaFuncAttributes fa;
-      MGV_CUDA_TRY(cudaDeviceGetAttribute(&optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, pl.device));
-      MGV_CUDA_TRY(cudaFuncGetAttributes(&fa, KERN));
-      MGV_CUDA_TRY(cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, optin - int(fa.sharedSizeBytes)));
-      configured[pl.device] = true;
-    }
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(pl.grid);
-  cfg.blockDim = dim3(kGemmThreads);
-  cfg.dynamicSmemBytes = pl.smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attrs[2];
-  int n = 0;
-  if (pl.p.split > 1) {
-    attrs[n].id = cudaLaunchAttributeClusterDimension;
-    attrs[n].val.clusterDim.x = unsigned(pl.p.split);
-    attrs[n].val.clusterDim.y = attrs[n].val.clusterDim.z = 1;
-    ++n;
-  }
-  if (pl.flags & MGV_FLAG_PDL) {
-    attrs[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attrs[n].val.programmaticStreamSerializationAllowed = 1;
-    ++n;
-  }
-  cfg.attrs = attrs;
-  cfg.numAttrs = n;
-  MGV_CUDA_TRY(cudaLaunchKernelEx(&cfg, KERN, pl.p));
-  return MGV_STATUS_OK;
+  return encode_rows(&p.x_map, a->x, a->M, a->K, a->ldx, pl.pair ? p.bt / 2 : p.bt);
 }
 
 template <int ACT>
-static mgv_status launch_act(const mgv_gemm_i8_plan &pl, cudaStream_t s) {
-  return pl.bf16 ? launch_kernel<gemm_i8_block_kernel<ACT, true>>(pl, s) : launch_kernel<gemm_i8_block_kernel<ACT, false>>(pl, s);
+static mgv_status launch_act(const GemmI8Plan &pl, cudaStream_t s) {
+  return pl.bf16 ? launch_gemm<gemm_i8_block_kernel<ACT, true>>(pl, s) : launch_gemm<gemm_i8_block_kernel<ACT, false>>(pl, s);
 }
 
-static mgv_status launch(const mgv_gemm_i8_plan &pl, cudaStream_t s) {
+static mgv_status launch(const GemmI8Plan &pl, cudaStream_t s) {
   if (pl.p.M == 0) return MGV_STATUS_OK;
+  if (pl.pair) return launch_gemm_pair(pl, s);
   switch (pl.act) {
     case kActRelu: return launch_act<kActRelu>(pl, s);
     case kActSilu: return launch_act<kActSilu>(pl, s);

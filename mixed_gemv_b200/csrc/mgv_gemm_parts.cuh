@@ -4,6 +4,8 @@
 #include <cuda.h>  // CUtensorMap (types only: the encoder is looked up at run time)
 #include <cuda_bf16.h>
 
+#include <mutex>
+
 #include "mgv_common.cuh"
 
 namespace mgv {
@@ -22,7 +24,7 @@ struct GemmI8Params {
   int bt;          // activation rows of a tile
   int stages;      // ring slots
   int split;       // blocks of a cluster that share a tile's K range
-  int n_tiles;
+  int n_tiles, m_tiles;
   uint32_t idesc;  // instruction descriptor of the matrix instruction
   uint32_t tmem_cols;
 };
@@ -73,6 +75,14 @@ __device__ __forceinline__ void box_load(uint32_t dst, const CUtensorMap *map, i
                : "memory");
 }
 
+// The same from one block of a pair that works on a common tile: bytes are counted on a barrier of
+// either block (an address in the cluster's window).
+__device__ __forceinline__ void box_load_pair(uint32_t dst, const CUtensorMap *map, int k, int row, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(k), "r"(row), "r"(bar)
+               : "memory");
+}
+
 // Shared-memory operand descriptor: rows of 128 bytes along K in the 128-byte swizzle, groups of
 // eight rows 1024 bytes apart.
 __device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
@@ -105,6 +115,15 @@ __device__ __forceinline__ uint32_t in_block(uint32_t addr, uint32_t rank) {
   uint32_t r;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
+}
+__device__ __forceinline__ void arrive_in_block(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Arrives at the barrier `bar` of both blocks of a pair when the matrix instructions issued so far have completed.
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+               "h"(uint16_t(3))
+               : "memory");
 }
 __device__ __forceinline__ int load_cluster(uint32_t addr) {
   int v;
@@ -174,5 +193,57 @@ __device__ __forceinline__ void finish_pair(const GemmI8Params &p, const Feature
 }
 
 #endif  // __CUDACC__
+
+// ---- host side, shared by the translation units ----
+
+struct GemmI8Plan {
+  GemmI8Params p;
+  int device = 0, grid = 0, smem = 0, cluster = 1, act = 0, bf16 = 0, flags = 0;
+  int pair = 0;  // the kernel of block pairs takes the call
+};
+
+// Launches KERN as the plan says; its first launch on a device lifts its shared-memory limit.
+template <auto KERN>
+mgv_status launch_gemm(const GemmI8Plan &pl, cudaStream_t s) {
+  static bool configured[64];
+  static std::mutex mu;
+  if (pl.device < 0 || pl.device >= 64) return fail(MGV_STATUS_UNSUPPORTED, "gemm_i8: device index %d beyond 63", pl.device);
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (!configured[pl.device]) {
+      int optin = 0;
+      cudaFuncAttributes fa;
+      MGV_CUDA_TRY(cudaDeviceGetAttribute(&optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, pl.device));
+      MGV_CUDA_TRY(cudaFuncGetAttributes(&fa, KERN));
+      MGV_CUDA_TRY(cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, optin - int(fa.sharedSizeBytes)));
+      configured[pl.device] = true;
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(pl.grid);
+  cfg.blockDim = dim3(kGemmThreads);
+  cfg.dynamicSmemBytes = pl.smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attrs[2];
+  int n = 0;
+  if (pl.cluster > 1) {
+    attrs[n].id = cudaLaunchAttributeClusterDimension;
+    attrs[n].val.clusterDim.x = unsigned(pl.cluster);
+    attrs[n].val.clusterDim.y = attrs[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (pl.flags & MGV_FLAG_PDL) {
+    attrs[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attrs;
+  cfg.numAttrs = n;
+  MGV_CUDA_TRY(cudaLaunchKernelEx(&cfg, KERN, pl.p));
+  return MGV_STATUS_OK;
+}
+
+// The kernel of block pairs (mgv_gemm_pair.cu).
+mgv_status launch_gemm_pair(const GemmI8Plan &pl, cudaStream_t s);
 
 }  // namespace mgv

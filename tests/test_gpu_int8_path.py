@@ -240,6 +240,27 @@ def test_gemm(cuda_lib, M, N, K, act):
     Product(M, N, K, torch.bfloat16 if M % 2 else torch.float16, bias=N % 4 == 0, act=act, seed=M).run().check()
 
 
+PATHS = [_lib.GEMM_HINT_BLOCK | _lib.gemm_hint_split(s) | _lib.gemm_hint_rows(r) for s in (1, 2, 4, 8) for r in (16, 96, 256)] + \
+        [_lib.GEMM_HINT_PAIR | _lib.gemm_hint_rows(r) for r in (32, 96, 160, 256)]
+
+
+@pytest.mark.parametrize("hints", PATHS)
+@pytest.mark.parametrize("M, N, K, act", [(1, 100, 64, "none"), (77, 300, 1300, "silu"), (500, 642, 2049, "gated"), (513, 1025, 2000, "relu")])
+def test_every_kernel_and_tiling_gives_the_same_bits(cuda_lib, M, N, K, act, hints):
+    p = Product(M, N, K, act=act, bias=True, seed=6).run(hints=hints).check()
+    forced = p.out.clone()
+    assert torch.equal(p.run().out, forced)
+    assert api.device_error_state() == 0
+
+
+def test_more_tiles_than_blocks(cuda_lib):
+    """Every pair of blocks takes several tiles, whose accumulators and ring slots alternate."""
+    for M, N, K in ((2000, 5000, 200), (4096, 8192, 1100)):
+        for rows in (64, 256):
+            Product(M, N, K, act="gated", seed=7).run(hints=_lib.GEMM_HINT_PAIR | _lib.gemm_hint_rows(rows)).check()
+    assert api.device_error_state() == 0
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("scales", [torch.float16, torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("act", list(ACTS))

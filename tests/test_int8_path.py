@@ -82,7 +82,8 @@ def test_norm_refusals(kw, status):
 @pytest.mark.parametrize("kw, status", [
     (dict(struct_size=8), Status.INVALID_ARGUMENT),
     (dict(M=-1), Status.INVALID_ARGUMENT),
-    (dict(M=1 << 31), Status.INVALID_ARGUMENT),
+    (dict(M=(1 << 30) + 1), Status.INVALID_ARGUMENT),
+    (dict(N=(1 << 30) + 1, ldd=1 << 31), Status.INVALID_ARGUMENT),
     (dict(N=0), Status.INVALID_ARGUMENT),
     (dict(K=0), Status.INVALID_ARGUMENT),
     (dict(K=131072, ldx=131072, ldw=131072), Status.INVALID_ARGUMENT),
