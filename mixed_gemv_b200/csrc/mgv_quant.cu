@@ -2,6 +2,7 @@
 // norm with the residual's addition, and the way back.
 #include <cuda_bf16.h>
 
+#include <algorithm>
 #include <cfloat>
 #include <cmath>
 
@@ -19,8 +20,6 @@ struct RowParams {
   float eps;
 };
 
-constexpr int kRowThreads = 256;
-
 __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <typename T>
@@ -30,74 +29,383 @@ __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-template <typename V>
-__device__ __forceinline__ V block_reduce(V v, V (*op)(V, V), V *buf) {
-  for (int o = 16; o; o >>= 1) v = op(v, __shfl_xor_sync(~0u, v, o));
+// Two values of a 32-bit word, and back (each rounded to T).
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t u);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2 *>(&u)); }
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// What a thread holds of a row at a time: eight neighbouring 16-bit values in four words (V = 8, one
+// 16-byte access), or one value, the low half of a word whose high half is zero (V = 1).
+template <int V>
+struct Piece {
+  uint32_t u[V == 8 ? 4 : 1];
+};
+// Of a piece at `at`, `n` values belong to the row: what is behind its end is neither read (it counts
+// as zero) nor written.
+template <int V>
+__device__ __forceinline__ Piece<V> load_piece(const void *row, int k, int n) {
+  const uint16_t *at = static_cast<const uint16_t *>(row) + k;
+  Piece<V> r;
+  if constexpr (V == 1) {
+    r.u[0] = *at;
+  } else if (n >= 8) {
+    const uint4 v = *reinterpret_cast<const uint4 *>(at);
+    r.u[0] = v.x, r.u[1] = v.y, r.u[2] = v.z, r.u[3] = v.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r.u[j] = (2 * j < n ? uint32_t(at[2 * j]) : 0u) | (2 * j + 1 < n ? uint32_t(at[2 * j + 1]) << 16 : 0u);
+  }
+  return r;
+}
+template <int V>
+__device__ __forceinline__ void store_piece(void *row, int k, const Piece<V> &v, int n) {
+  uint16_t *at = static_cast<uint16_t *>(row) + k;
+  if constexpr (V == 1) {
+    *at = uint16_t(v.u[0]);
+  } else if (n >= 8) {
+    *reinterpret_cast<uint4 *>(at) = make_uint4(v.u[0], v.u[1], v.u[2], v.u[3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) at[j] = uint16_t(v.u[j / 2] >> (j % 2 * 16));
+  }
+}
+
+// Four fp32 values in [-127, 127], each added to 1.5 * 2^23 (so rounded to an integer, ties to even):
+// the low bytes are the integers.
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
+  const uint32_t ab = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040);
+  const uint32_t cd = __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040);
+  return __byte_perm(ab, cd, 0x5410);
+}
+constexpr float kRoundMagic = 12582912.0f;
+
+__device__ __forceinline__ double block_reduce_double(double v, bool largest, double *buf) {
+  for (int o = 16; o; o >>= 1) {
+    const double w = __shfl_xor_sync(~0u, v, o);
+    v = largest ? fmax(v, w) : v + w;
+  }
+  __syncthreads();
   if (threadIdx.x % 32 == 0) buf[threadIdx.x / 32] = v;
   __syncthreads();
   v = buf[0];
-  for (int i = 1; i < kRowThreads / 32; ++i) v = op(v, buf[i]);
-  __syncthreads();
+  for (int i = 1; i < int(blockDim.x / 32); ++i) v = largest ? fmax(v, buf[i]) : v + buf[i];
   return v;
 }
 
-// One block per row, two passes.  Double precision throughout: right for every finite row,
-// whatever its magnitude.
-template <typename T, bool NORM>
-__global__ void __launch_bounds__(kRowThreads) rows_kernel(RowParams p) {
-  __shared__ double buf[kRowThreads / 32];
-  const int64_t m = blockIdx.x;
-  const T *x = static_cast<const T *>(p.x) + m * p.ldx;
-  const T *r = p.residual ? static_cast<const T *>(p.residual) + m * p.ldr : nullptr;
-  T *ro = p.residual ? static_cast<T *>(p.residual_out) + m * p.ldro : nullptr;
+// One row in double precision, by `step` threads from `t`: right for whatever magnitude its values
+// have.  The kernels come here for a row that has no finite fp32 statistics (an infinity or a NaN
+// among the values, squares or products beyond fp32, or all of them near its smallest), and re-read
+// the row, with the residual already added.
+template <typename T, bool NORM, bool WARP_ROW>
+__device__ __noinline__ void row_in_double(const RowParams &p, int64_t m, int t, int step, double *buf) {
+  const T *h = p.residual ? static_cast<const T *>(p.residual_out) + m * p.ldro : static_cast<const T *>(p.x) + m * p.ldx;
   const T *w = static_cast<const T *>(p.weight);
   int8_t *q = p.q + m * p.ldq;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  double ss = 0, top = 0;
-  bool bad = false;
-  for (int k = threadIdx.x; k < p.K; k += kRowThreads) {
-    float h = to_f(x[k]);
-    if (NORM && r) {
-      const T t = from_f<T>(h + to_f(r[k]));
-      ro[k] = t;
-      h = to_f(t);
-    }
-    const double v = NORM ? double(h) * double(to_f(w[k])) : double(h);
-    bad |= !(fabs(v) <= DBL_MAX);
-    ss += double(h) * double(h);
-    top = fmax(top, fabs(v));
+  if (WARP_ROW) __syncwarp();
+  else __syncthreads();  // the row's threads have stored their part of residual_out, and read the mark in scale
+  double ss = 0, top = 0, bad = 0;
+  for (int k = t; k < p.K; k += step) {
+    const double v = to_f(h[k]), y = NORM ? v * double(to_f(w[k])) : v;
+    if (!(fabs(y) <= DBL_MAX)) bad = 1;
+    ss += v * v;
+    top = fmax(top, fabs(y));
   }
-  auto add = [](double a, double b) { return a + b; };
-  auto larger = [](double a, double b) { return fmax(a, b); };
-  if (NORM) ss = block_reduce<double>(ss, add, buf);
-  top = block_reduce<double>(top, larger, buf);
-  bad = block_reduce<double>(bad ? 1.0 : 0.0, larger, buf) != 0.0;
+  if (WARP_ROW) {
+    for (int o = 16; o; o >>= 1) {
+      ss += __shfl_xor_sync(~0u, ss, o);
+      top = fmax(top, __shfl_xor_sync(~0u, top, o));
+      bad = fmax(bad, __shfl_xor_sync(~0u, bad, o));
+    }
+  } else {
+    ss = block_reduce_double(ss, false, buf);
+    top = block_reduce_double(top, true, buf);
+    bad = block_reduce_double(bad, true, buf);
+  }
   const double inv = top > 0 ? 127.0 / top : 0.0;
-  if (threadIdx.x == 0) {
+  if (t == 0) {
     double s = top / 127.0;
     if (NORM && top > 0) s /= sqrt(ss / p.K + double(p.eps));
-    p.scale[m] = bad ? NAN : float(s);
+    p.scale[m] = bad != 0 ? NAN : float(s);
   }
-  const T *again = NORM && r ? ro : x;
-  for (int k = threadIdx.x; k < p.K; k += kRowThreads) {
-    const double v = NORM ? double(to_f(again[k])) * double(to_f(w[k])) : double(to_f(again[k]));
-    q[k] = bad ? 0 : int8_t(rint(v * inv));
+  for (int k = t; k < p.K; k += step) {
+    const double v = to_f(h[k]), y = NORM ? v * double(to_f(w[k])) : v;
+    q[k] = bad != 0 ? 0 : int8_t(rint(y * inv));
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) back_kernel(T *out, const int8_t *q, const float *scale, int K, int64_t ldo, int64_t ldq) {
-  const int64_t m = blockIdx.x;
+// Statistics of a row: the sum of squares of h, and the largest |h w| as the bits of a float (whose
+// order as integers is that of the magnitudes, with infinities and NaN above every number).
+struct RowStats {
+  float ss;
+  uint32_t top;
+};
+// The fp32 statistics serve: squares, products and their quotients are numbers well inside fp32.
+template <bool NORM>
+__device__ __forceinline__ bool row_is_tame(const RowParams &p, const RowStats &s, float mean) {
+  const bool sum_ok = !NORM || (mean >= 1e-30f && mean <= FLT_MAX);
+  return sum_ok && (s.top == 0 || (s.top >= __float_as_uint(1e-30f) && s.top < 0x7f800000u));
+}
+template <bool NORM>
+__device__ __forceinline__ void row_factors(const RowStats &s, float mean, float &scale, float &inv) {
+  const float top = __uint_as_float(s.top);
+  scale = (NORM ? top * rsqrtf(mean) : top) / 127.0f;
+  inv = s.top ? 127.0f / top : 0.0f;
+}
+__device__ __forceinline__ RowStats warp_stats(RowStats s) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s.ss += __shfl_xor_sync(~0u, s.ss, o);
+  s.top = __reduce_max_sync(~0u, s.top);
+  return s;
+}
+__device__ __forceinline__ RowStats block_stats(RowStats s, RowStats *buf) {
+  s = warp_stats(s);
+  if (threadIdx.x % 32 == 0) buf[threadIdx.x / 32] = s;
+  __syncthreads();
+  const int warps = blockDim.x / 32, lane = threadIdx.x % 32;
+  RowStats r = {0.0f, 0u};
+  if (lane < warps) r = buf[lane];
+  return warp_stats(r);
+}
+
+// Marks, in its place in `scale`, a row that is left for row_in_double.
+constexpr float kLeft = -1.0f;
+
+// The rows in one pass.  A row's h stays in registers, 16 bits a value, between the statistics and the
+// quantisation, and one reduction serves both: with y = h w r, r = 1 / sqrt(mean + eps), the scale is
+// r max|h w| / 127 and q = h w 127 / max|h w|, in which r does not occur.  The sum of squares, the
+// largest value and the scale are fp32.  A block takes a row (a warp, for short rows) with NV pieces of V
+// values to a thread, then the next one; the norm's weights stay in registers over its rows.
+template <typename T, bool NORM, int V, int NV, bool WARP_ROW>
+__global__ void __launch_bounds__(WARP_ROW ? 128 : 1024, WARP_ROW ? 6 : 1) rows_kernel(const __grid_constant__ RowParams p) {
+  constexpr bool kKeepWeight = NV <= 2;
+  constexpr int kWords = V == 8 ? 4 : 1;
+  using P = Piece<V>;
+  __shared__ RowStats stats[2][32];
+  __shared__ double buf[32];
+  const int step = WARP_ROW ? 32 : blockDim.x, t = WARP_ROW ? threadIdx.x % 32 : threadIdx.x;
+  const int per_block = WARP_ROW ? 4 : 1;
+  const int64_t first = int64_t(blockIdx.x) * per_block + (WARP_ROW ? threadIdx.x / 32 : 0), stride = int64_t(gridDim.x) * per_block;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  P w[NORM && kKeepWeight ? NV : 1];
+  if (NORM && kKeepWeight) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int k = (i * step + t) * V;
+      if (k < p.K) w[i] = load_piece<V>(p.weight, k, p.K - k);
+    }
+  }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const float s = scale[m];
-  for (int k = threadIdx.x; k < K; k += kRowThreads) out[m * ldo + k] = from_f<T>(float(q[m * ldq + k]) * s);
+  int turn = 0;
+  bool left = false;
+  for (int64_t m = first; m < p.M; m += stride, turn ^= 1) {
+    const T *x = static_cast<const T *>(p.x) + m * p.ldx;
+    P h[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int k = (i * step + t) * V;
+      if (k < p.K) h[i] = load_piece<V>(x, k, p.K - k);
+    }
+    if (NORM && p.residual) {
+      const T *r = static_cast<const T *>(p.residual) + m * p.ldr;
+      T *ro = static_cast<T *>(p.residual_out) + m * p.ldro;
+      constexpr int kGroup = NV < 4 ? NV : 4;  // loads in flight, within the registers there are
+      P add[kGroup];
+#pragma unroll
+      for (int g = 0; g < NV; g += kGroup) {
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) {
+          const int k = ((g + i) * step + t) * V;
+          if (k < p.K) add[i] = load_piece<V>(r, k, p.K - k);
+        }
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) {
+          const int k = ((g + i) * step + t) * V;
+          if (k < p.K) {
+#pragma unroll
+            for (int j = 0; j < kWords; ++j) {
+              const float2 a = unpack2<T>(h[g + i].u[j]), b = unpack2<T>(add[i].u[j]);
+              h[g + i].u[j] = pack2<T>(a.x + b.x, a.y + b.y);
+            }
+            store_piece<V>(ro, k, h[g + i], p.K - k);
+          }
+        }
+      }
+    }
+    RowStats s = {0.0f, 0u};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int k = (i * step + t) * V;
+      if (k < p.K) {
+        P wi = {};
+        if (NORM) wi = kKeepWeight ? w[kKeepWeight ? i : 0] : load_piece<V>(p.weight, k, p.K - k);
+#pragma unroll
+        for (int j = 0; j < kWords; ++j) {
+          const float2 v = unpack2<T>(h[i].u[j]);
+          float2 y = v;
+          if (NORM) {
+            const float2 g = unpack2<T>(wi.u[j]);
+            y = make_float2(v.x * g.x, v.y * g.y);
+            s.ss = fmaf(v.x, v.x, s.ss);
+            s.ss = fmaf(v.y, v.y, s.ss);
+          }
+          s.top = max(s.top, max(__float_as_uint(y.x) & 0x7fffffffu, __float_as_uint(y.y) & 0x7fffffffu));
+        }
+      }
+    }
+    s = WARP_ROW ? warp_stats(s) : block_stats(s, stats[turn]);
+    const float mean = s.ss / float(p.K) + p.eps;
+    if (!row_is_tame<NORM>(p, s, mean)) {
+      if (t == 0) p.scale[m] = kLeft;
+      left = true;
+      continue;
+    }
+    float scale, inv;
+    row_factors<NORM>(s, mean, scale, inv);
+    if (t == 0) p.scale[m] = scale;
+    int8_t *q = p.q + m * p.ldq;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int k = (i * step + t) * V;
+      if (k < p.K) {
+        P wi = {};
+        if (NORM) wi = kKeepWeight ? w[kKeepWeight ? i : 0] : load_piece<V>(p.weight, k, p.K - k);
+        float2 y[kWords];
+#pragma unroll
+        for (int j = 0; j < kWords; ++j) {
+          float2 v = unpack2<T>(h[i].u[j]);
+          if (NORM) {
+            const float2 g = unpack2<T>(wi.u[j]);
+            v = make_float2(v.x * g.x, v.y * g.y);
+          }
+          y[j] = make_float2(fmaf(v.x, inv, kRoundMagic), fmaf(v.y, inv, kRoundMagic));
+        }
+        if constexpr (V == 8) {
+          const uint2 o = make_uint2(pack4(y[0].x, y[0].y, y[1].x, y[1].y), pack4(y[2].x, y[2].y, y[3].x, y[3].y));
+          const int n = p.K - k;
+          if (n >= 8) *reinterpret_cast<uint2 *>(q + k) = o;
+          else
+            for (int j = 0; j < n; ++j) q[k + j] = int8_t((j < 4 ? o.x : o.y) >> (j % 4 * 8));
+        } else {
+          q[k] = int8_t(__float_as_uint(y[0].x) & 0xff);
+        }
+      }
+    }
+  }
+  if (!left) return;  // the same for all threads of a row
+  if (WARP_ROW) __syncwarp();
+  else __syncthreads();
+  for (int64_t m = first; m < p.M; m += stride)
+    if (*static_cast<volatile float *>(p.scale + m) == kLeft) row_in_double<T, NORM, WARP_ROW>(p, m, t, step, buf);
+}
+
+// Rows too long for registers: a block per row, value by value, in two passes over it.
+template <typename T, bool NORM>
+__global__ void __launch_bounds__(1024, 1) long_rows_kernel(const __grid_constant__ RowParams p) {
+  __shared__ RowStats stats[32];
+  __shared__ double buf[32];
+  const int64_t m = blockIdx.x;
+  const T *x = static_cast<const T *>(p.x) + m * p.ldx, *w = static_cast<const T *>(p.weight);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const T *h = x;
+  RowStats s = {0.0f, 0u};
+  if (NORM && p.residual) {
+    const T *r = static_cast<const T *>(p.residual) + m * p.ldr;
+    T *ro = static_cast<T *>(p.residual_out) + m * p.ldro;
+    for (int k = threadIdx.x; k < p.K; k += blockDim.x) ro[k] = from_f<T>(to_f(x[k]) + to_f(r[k]));
+    h = ro;  // every thread reads back what it wrote
+  }
+#pragma unroll 4
+  for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
+    const float v = to_f(h[k]), y = NORM ? v * to_f(w[k]) : v;
+    if (NORM) s.ss = fmaf(v, v, s.ss);
+    s.top = max(s.top, __float_as_uint(y) & 0x7fffffffu);
+  }
+  s = block_stats(s, stats);
+  const float mean = s.ss / float(p.K) + p.eps;
+  if (!row_is_tame<NORM>(p, s, mean)) {
+    row_in_double<T, NORM, false>(p, m, threadIdx.x, blockDim.x, buf);
+    return;
+  }
+  float scale, inv;
+  row_factors<NORM>(s, mean, scale, inv);
+  if (threadIdx.x == 0) p.scale[m] = scale;
+  int8_t *q = p.q + m * p.ldq;
+#pragma unroll 4
+  for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
+    const float v = to_f(h[k]);
+    q[k] = int8_t(__float_as_uint(fmaf(NORM ? v * to_f(w[k]) : v, inv, kRoundMagic)) & 0xff);
+  }
+}
+
+struct BackParams {
+  const int8_t *q;
+  const float *scale;
+  void *out;
+  int64_t M, ldq, ldo;
+  int K, lanes;  // lanes: threads of a block that share a row, a power of two
+};
+
+constexpr int kBackThreads = 256;
+
+// One piece of V values per thread and row group; a block takes kBackThreads / lanes rows at a time.
+template <typename T, int V>
+__global__ void __launch_bounds__(kBackThreads) back_kernel(const BackParams p) {
+  const int rows = kBackThreads / p.lanes, row = threadIdx.x / p.lanes, width = p.lanes * V;
+  const int64_t chunks = (p.K + width - 1) / width;
+  const int64_t m = int64_t(blockIdx.x / chunks) * rows + row;
+  const int k = int(blockIdx.x % chunks) * width + (threadIdx.x % p.lanes) * V;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (m >= p.M || k >= p.K) return;
+  const int n = p.K - k;
+  const float s = p.scale[m];
+  T *out = static_cast<T *>(p.out) + m * p.ldo + k;
+  const int8_t *q = p.q + m * p.ldq + k;
+  if (V == 16 && n >= V) {
+    const uint4 b = *reinterpret_cast<const uint4 *>(q);
+    const uint32_t word[4] = {b.x, b.y, b.z, b.w};
+    uint32_t o[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float f[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)  // q + 128 in the mantissa of 2^23: exact, without a conversion instruction
+        f[j] = (__uint_as_float(__byte_perm(word[i] ^ 0x80808080u, 0x4b000000u, 0x7540 + j)) - 8388736.0f) * s;
+      o[2 * i] = pack2<T>(f[0], f[1]);
+      o[2 * i + 1] = pack2<T>(f[2], f[3]);
+    }
+    reinterpret_cast<uint4 *>(out)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+    reinterpret_cast<uint4 *>(out)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+  } else {
+    for (int j = 0; j < V && j < n; ++j) out[j] = from_f<T>(float(q[j]) * s);
+  }
 }
 
 template <typename... P, typename... A>
-static mgv_status launch_rows(void (*kern)(P...), int64_t rows, int flags, cudaStream_t s, A... a) {
+static mgv_status launch_rows(void (*kern)(P...), int64_t grid, int threads, int flags, cudaStream_t s, A... a) {
+  if (grid > 0x7fffffff) return fail(MGV_STATUS_UNSUPPORTED, "row kernel: too many rows for one launch");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(rows));
-  cfg.blockDim = dim3(kRowThreads);
+  cfg.gridDim = dim3(unsigned(grid));
+  cfg.blockDim = dim3(unsigned(threads));
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -106,6 +414,62 @@ static mgv_status launch_rows(void (*kern)(P...), int64_t rows, int flags, cudaS
   cfg.numAttrs = (flags & MGV_FLAG_PDL) ? 1 : 0;
   MGV_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, a...));
   return MGV_STATUS_OK;
+}
+
+static bool aligned_rows(const void *p, int64_t ld, int64_t elem, int64_t rows, unsigned to) {
+  return reinterpret_cast<uintptr_t>(p) % to == 0 && (rows <= 1 || ld * elem % to == 0);
+}
+
+static int sm_count() {
+  static int count[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (!count[dev] && cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) count[dev] = 0;
+  return count[dev] ? count[dev] : 148;
+}
+
+template <typename T, bool NORM>
+static mgv_status quantise(const RowParams &p, int flags, cudaStream_t s) {
+  const bool wide = aligned_rows(p.x, p.ldx, 2, p.M, 16) && aligned_rows(p.q, p.ldq, 1, p.M, 8) &&
+                    (!NORM || (aligned_rows(p.weight, 0, 2, 1, 16) &&
+                               (!p.residual || (aligned_rows(p.residual, p.ldr, 2, p.M, 16) && aligned_rows(p.residual_out, p.ldro, 2, p.M, 16)))));
+  const int sms = sm_count();
+  if (wide && p.K <= 65536) {
+    const int pieces = (p.K + 7) / 8;
+    const int64_t few = 2 * int64_t(sms);
+    if (pieces <= 128 && p.M > few)
+      return launch_rows(rows_kernel<T, NORM, 8, 4, true>, std::min<int64_t>((p.M + 3) / 4, int64_t(sms) * 16), 128, flags, s, p);
+    // few rows: as many threads as a row has pieces, for the shortest chain of loads; many rows: four pieces a
+    // thread, so that several blocks of an SM are at different points of their rows
+    int nv = 1;
+    while (nv < 8 && pieces > 1024 * nv) nv *= 2;
+    if (p.M > few) nv = std::max(nv, 4);
+    const int threads = std::max(32, ((pieces + nv - 1) / nv + 31) / 32 * 32);
+    const int64_t grid = std::min<int64_t>(p.M, int64_t(sms) * std::max(1, 2048 / threads));
+    switch (nv) {
+      case 1: return launch_rows(rows_kernel<T, NORM, 8, 1, false>, grid, threads, flags, s, p);
+      case 2: return launch_rows(rows_kernel<T, NORM, 8, 2, false>, grid, threads, flags, s, p);
+      case 4: return launch_rows(rows_kernel<T, NORM, 8, 4, false>, grid, threads, flags, s, p);
+      default: return launch_rows(rows_kernel<T, NORM, 8, 8, false>, grid, threads, flags, s, p);
+    }
+  }
+  if (p.K <= 8192) {
+    const int threads = std::max(32, ((p.K + 7) / 8 + 31) / 32 * 32);
+    const int64_t grid = std::min<int64_t>(p.M, int64_t(sms) * std::max(1, 2048 / threads));
+    return launch_rows(rows_kernel<T, NORM, 1, 8, false>, grid, threads, flags, s, p);
+  }
+  return launch_rows(long_rows_kernel<T, NORM>, p.M, 1024, flags, s, p);
+}
+
+template <typename T>
+static mgv_status dequantise(BackParams p, int flags, cudaStream_t s) {
+  const bool wide = aligned_rows(p.q, p.ldq, 1, p.M, 16) && aligned_rows(p.out, p.ldo, 2, p.M, 16);
+  const int v = wide ? 16 : 1;
+  p.lanes = 1;
+  while (p.lanes < kBackThreads && p.lanes * v < p.K) p.lanes *= 2;
+  const int rows = kBackThreads / p.lanes;
+  const int64_t grid = (p.M + rows - 1) / rows * ((p.K + p.lanes * v - 1) / (p.lanes * v));
+  return wide ? launch_rows(back_kernel<T, 16>, grid, kBackThreads, flags, s, p) : launch_rows(back_kernel<T, 1>, grid, kBackThreads, flags, s, p);
 }
 
 // What the three entry points check alike; `what` names the call in the message.
@@ -146,8 +510,7 @@ extern "C" mgv_status mgv_quantize_rows(void *q, void *scale, const void *x, int
   RowParams p = {};
   p.x = x; p.q = static_cast<int8_t *>(q); p.scale = static_cast<float *>(scale);
   p.M = M; p.K = K; p.ldx = ldx; p.ldq = ldq;
-  return dtype == MGV_DTYPE_F16 ? launch_rows(rows_kernel<__half, false>, M, flags, s, p)
-                                : launch_rows(rows_kernel<__nv_bfloat16, false>, M, flags, s, p);
+  return dtype == MGV_DTYPE_F16 ? quantise<__half, false>(p, flags, s) : quantise<__nv_bfloat16, false>(p, flags, s);
 }
 
 extern "C" mgv_status mgv_dequantize_rows(void *out, const void *q, const void *scale, int dtype, int64_t M, int32_t K,
@@ -157,10 +520,10 @@ extern "C" mgv_status mgv_dequantize_rows(void *out, const void *q, const void *
   MGV_CHECK(check_operand("dequantize_rows", "out", out, ldo, K, 2));
   MGV_CHECK(check_operand("dequantize_rows", "q", q, ldq, K, 1));
   MGV_CHECK(check_operand("dequantize_rows", "scale", scale, K, K, 4));
-  const int8_t *qp = static_cast<const int8_t *>(q);
-  const float *sp = static_cast<const float *>(scale);
-  return dtype == MGV_DTYPE_F16 ? launch_rows(back_kernel<__half>, M, flags, s, static_cast<__half *>(out), qp, sp, K, ldo, ldq)
-                                : launch_rows(back_kernel<__nv_bfloat16>, M, flags, s, static_cast<__nv_bfloat16 *>(out), qp, sp, K, ldo, ldq);
+  BackParams p = {};
+  p.q = static_cast<const int8_t *>(q); p.scale = static_cast<const float *>(scale); p.out = out;
+  p.M = M; p.K = K; p.ldq = ldq; p.ldo = ldo;
+  return dtype == MGV_DTYPE_F16 ? dequantise<__half>(p, flags, s) : dequantise<__nv_bfloat16>(p, flags, s);
 }
 
 extern "C" void mgv_rmsnorm_args_init(mgv_rmsnorm_args *a) {
@@ -191,6 +554,5 @@ extern "C" mgv_status mgv_rmsnorm_quantize(const mgv_rmsnorm_args *a, mgv_stream
   p.x = a->x; p.residual = a->residual; p.weight = a->weight; p.residual_out = a->residual_out;
   p.q = static_cast<int8_t *>(a->q); p.scale = static_cast<float *>(a->scale);
   p.M = a->M; p.K = a->K; p.ldx = a->ldx; p.ldr = a->ldr; p.ldro = a->ldro; p.ldq = a->ldq; p.eps = a->eps;
-  return a->dtype == MGV_DTYPE_F16 ? launch_rows(rows_kernel<__half, true>, a->M, a->flags, s, p)
-                                   : launch_rows(rows_kernel<__nv_bfloat16, true>, a->M, a->flags, s, p);
+  return a->dtype == MGV_DTYPE_F16 ? quantise<__half, true>(p, a->flags, s) : quantise<__nv_bfloat16, true>(p, a->flags, s);
 }
