@@ -403,8 +403,8 @@ typedef struct mgv_gemm_i8_args {
 
 /* Plan hints (mgv_gemm_i8_args.hints).  Every combination computes the same bits through another
  * kernel or tiling; they exist so that tests and tuning runs can reach each path on any shape.
- * Bits 0..2: blocks that share a tile's K range, as 1 + log2 (0: the library chooses).  Bits 8..12:
- * rows of x in a tile, in units of 16 (rounded up to what the kernel takes; 0: the library chooses). */
+ * Bits 8..12: rows of x in a tile, in units of 16 (rounded up to what the kernel takes; 0:
+ * the library chooses the tiling).  Bits 0..2, with those: blocks that share a tile's K range, less 1. */
 enum {
   MGV_GEMM_HINT_BLOCK = 8,  /* the kernel of single blocks (small batches)                        */
   MGV_GEMM_HINT_PAIR = 16   /* the kernel of block pairs (prompts)                                */

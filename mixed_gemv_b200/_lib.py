@@ -83,7 +83,7 @@ GEMM_HINT_BLOCK, GEMM_HINT_PAIR = 8, 16
 
 
 def gemm_hint_split(blocks: int) -> int:
-    return blocks.bit_length()
+    return blocks - 1
 
 
 def gemm_hint_rows(rows: int) -> int:

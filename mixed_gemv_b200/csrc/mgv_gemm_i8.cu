@@ -12,18 +12,14 @@ namespace mgv {
 // column operand, whose width goes from 16 up: one token costs a sixteen-column tile, not 128 rows.
 // Weights and activations reach a ring of shared-memory slots by tiled bulk copies, one thread issues
 // the matrix instructions, accumulators are 32-bit integers in tensor memory: lane = feature, column =
-// row of the activations.  With split > 1 every block leaves its sums in shared memory and block r
-// adds and finishes the r-th part of the columns out of all of them; integer sums, so the result
-// does not depend on the split.
+// row of the activations.  With split > 1 every block sends each other one its sums of that block's share of the columns, and
+// adds and finishes its own share; integer sums, so the result does not depend on the split.
 template <int ACT, bool BF16>
 __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_block_kernel(const __grid_constant__ GemmI8Params p) {
   extern __shared__ uint8_t dynamic[];
-  __shared__ alignas(8) uint64_t full[kGemmMaxStages], empty[kGemmMaxStages], done;
-  __shared__ uint32_t tmem_base;
-  __shared__ int failed;
-  __shared__ alignas(16) float x_scale[256];
+  __shared__ GemmBlockShared sh;
   const uint32_t ring = (smem_u32(dynamic) + 1023) & ~1023u;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const uint32_t rank = p.split > 1 ? cluster_rank() : 0;
   const uint32_t tile = blockIdx.x / uint32_t(p.split);
   const int n0 = int(tile % uint32_t(p.n_tiles)) * kGemmRows, m0 = int(tile / uint32_t(p.n_tiles)) * p.bt;
@@ -32,68 +28,74 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_block_kernel(const __
   const uint32_t slot_bytes = kGemmABytes + p.bt * kGemmK;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < p.stages; ++i) bar_init(smem_u32(&full[i]), 1), bar_init(smem_u32(&empty[i]), 1);
-    bar_init(smem_u32(&done), 1);
-    failed = 0;
+    for (int i = 0; i < p.stages; ++i) bar_init(smem_u32(&sh.full[i]), 1), bar_init(smem_u32(&sh.empty[i]), 1);
+    bar_init(smem_u32(&sh.done), 1);
+    sh.failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(p.tmem_cols) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(p.tmem_cols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
-  const uint32_t tmem = tmem_base;
+  const uint32_t tmem = __shfl_sync(~0u, sh.tmem_base, 0);
   // only now: a dependent kernel that starts on this SM may hold tensor memory while it waits for this one to end
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {
     // weights of the first ring fill before the wait for the previous kernel, its output (x) after it
+    const bool one = elect_one();
     const int ahead = min(count, p.stages);
-    for (int i = 0; i < ahead; ++i) {
-      bar_expect(smem_u32(&full[i]), slot_bytes);
-      box_load(ring + i * slot_bytes, &p.w_map, (first + i) * kGemmK, n0, smem_u32(&full[i]));
+    if (one) {
+      for (int i = 0; i < ahead; ++i) {
+        bar_expect(smem_u32(&sh.full[i]), slot_bytes);
+        box_load(ring + i * slot_bytes, &p.w_map, (first + i) * kGemmK, n0, smem_u32(&sh.full[i]));
+      }
     }
     asm volatile("griddepcontrol.wait;\n\tfence.proxy.async.global;" ::: "memory");
-    for (int i = 0; i < ahead; ++i) box_load(ring + i * slot_bytes + kGemmABytes, &p.x_map, (first + i) * kGemmK, m0, smem_u32(&full[i]));
+    if (one)
+      for (int i = 0; i < ahead; ++i)
+        box_load(ring + i * slot_bytes + kGemmABytes, &p.x_map, (first + i) * kGemmK, m0, smem_u32(&sh.full[i]));
     int slot = 0, issued = ahead;
     uint32_t phase = 0;
-    for (int i = ahead; i < count; ++i) {
-      if (!bar_wait(smem_u32(&empty[slot]), phase, p.err)) break;
-      const uint32_t bar = smem_u32(&full[slot]), dst = ring + slot * slot_bytes;
-      bar_expect(bar, slot_bytes);
-      box_load(dst, &p.w_map, (first + i) * kGemmK, n0, bar);
-      box_load(dst + kGemmABytes, &p.x_map, (first + i) * kGemmK, m0, bar);
-      ++issued;
+    for (int i = ahead; i < count; ++i, ++issued) {
+      if (!bar_wait(smem_u32(&sh.empty[slot]), phase, p.err)) break;
+      if (one) {
+        const uint32_t bar = smem_u32(&sh.full[slot]), dst = ring + slot * slot_bytes;
+        bar_expect(bar, slot_bytes);
+        box_load(dst, &p.w_map, (first + i) * kGemmK, n0, bar);
+        box_load(dst + kGemmABytes, &p.x_map, (first + i) * kGemmK, m0, bar);
+      }
       if (++slot == p.stages) slot = 0, phase ^= 1;
     }
     // no copy may be in flight when the block ends: the last ones are waited for, whoever else gave up
     for (int i = max(0, issued - p.stages); i < issued; ++i)
-      if (!bar_wait(smem_u32(&full[i % p.stages]), (i / p.stages) & 1, p.err)) break;
-  } else if (warp == 1 && lane == 0) {
+      if (!bar_wait(smem_u32(&sh.full[i % p.stages]), (i / p.stages) & 1, p.err)) break;
+  } else if (warp == 1) {
+    const bool one = elect_one();
     int slot = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int i = 0; i < count && ok; ++i) {
-      ok = bar_wait(smem_u32(&full[slot]), phase, p.err);
+    for (int i = 0; i < count; ++i) {
+      ok = bar_wait(smem_u32(&sh.full[slot]), phase, p.err);
       if (!ok) break;
       tmem_fence_after();
       const uint64_t a = operand_desc(ring + slot * slot_bytes), b = operand_desc(ring + slot * slot_bytes + kGemmABytes);
+      if (one) {
 #pragma unroll
-      for (int k = 0; k < kGemmK / 32; ++k) {  // 32 bytes of K per instruction: two 16-byte steps of the descriptors
-        const uint32_t add = i + k > 0;
-        asm volatile(
-            "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, q;\n\t}" ::"r"(tmem),
-            "l"(a + 2 * k), "l"(b + 2 * k), "r"(p.idesc), "r"(add)
-            : "memory");
+        for (int k = 0; k < kGemmK / 32; ++k)  // 32 bytes of K per instruction: two 16-byte steps of the descriptors
+          multiply_add<1>(tmem, a + 2 * k, b + 2 * k, p.idesc, i + k > 0);
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&sh.empty[slot])) : "memory");
       }
-      asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&empty[slot])) : "memory");
+      __syncwarp();
       if (++slot == p.stages) slot = 0, phase ^= 1;
     }
-    if (!ok) *static_cast<volatile int *>(&failed) = 1;
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&done)) : "memory");
+    if (one) {
+      if (!ok) *static_cast<volatile int *>(&sh.failed) = 1;
+      asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&sh.done)) : "memory");
+    }
   }
 
   // tensor memory: a warp reads the 32 lanes of its number modulo 4
@@ -104,51 +106,57 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_block_kernel(const __
   if (warp >= 2) {
     f = load_feature<BF16>(p, n0 + row);
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    for (int i = threadIdx.x - 64; i < p.bt; i += 128) x_scale[i] = m0 + i < p.M ? p.x_scale[m0 + i] : 0.0f;
+    for (int i = threadIdx.x - 64; i < p.bt; i += 128) sh.x_scale[i] = m0 + i < p.M ? p.x_scale[m0 + i] : 0.0f;
     asm volatile("bar.sync 1, 128;" ::: "memory");
-    good = bar_wait(smem_u32(&done), 0, p.err) && !*static_cast<volatile int *>(&failed);
-    good = __all_sync(~0u, good);
+    good = bar_wait(smem_u32(&sh.done), 0, p.err) && !*static_cast<volatile int *>(&sh.failed);
     tmem_fence_after();
-    const int columns = min(p.bt, p.M - m0);
-    if (p.split == 1) {
-      if (good)
-        for (int c = 0; c < columns; c += 16) {
-          int v[16];
-          __syncwarp();
-          tmem_load16(lanes + c, v);
-          tmem_wait_load();
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) finish_pair<ACT, BF16>(p, f, m0 + c + i, v[i], v[i + 1], x_scale[c + i], x_scale[c + i + 1]);
-        }
-    } else {
-      // every copy has landed and every matrix instruction has read its slot: the ring's memory is free
+    if (p.split == 1 && good) {
+      const int columns = min(p.bt, p.M - m0);
       for (int c = 0; c < columns; c += 16) {
         int v[16];
+        __syncwarp();
         tmem_load16(lanes + c, v);
         tmem_wait_load();
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          asm volatile("st.shared.b32 [%0], %1;" ::"r"(ring + ((c + i) * kGemmRows + row) * 4), "r"(v[i]) : "memory");
+        finish16<ACT, BF16>(p, f, m0 + c, columns - c, v, sh.x_scale + c);
       }
     }
-    tmem_fence_before();
   }
   if (p.split > 1) {
+    // Every copy of the cluster has landed and every matrix instruction has read its slot: the rings'
+    // memory is free for the sums.  Block r finishes the 16-column groups r, r + split, ...; of each it
+    // gets, from each block, [4 quads of columns][128 features][4 columns].
+    cluster_sync();
+    const int groups = (min(p.bt, p.M - m0) + 15) / 16;
+    constexpr int kQuad = kGemmRows * 16, kGroup = 4 * kQuad;
+    if (warp >= 2) {
+      for (int g = 0; g < groups; ++g) {
+        int v[16];
+        __syncwarp();
+        tmem_load16(lanes + 16 * g, v);
+        tmem_wait_load();
+        const uint32_t to = in_block(ring, g % p.split) + ((g / p.split) * p.split + rank) * kGroup + row * 16;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) store_cluster(to + i * kQuad, v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+      }
+      tmem_fence_before();
+    }
     cluster_sync();
     if (warp >= 2 && good) {
-      const int share = p.bt / p.split, c0 = int(rank) * share, c1 = min(c0 + share, p.M - m0);
-      for (int c = c0; c < c1; c += 2) {
-        int a0 = 0, a1 = 0;
+      for (int g = int(rank); g < groups; g += p.split) {
+        const uint32_t from = ring + (g / p.split) * p.split * kGroup + row * 16;
+        int v[16] = {};
         for (int b = 0; b < p.split; ++b) {
-          const uint32_t at = in_block(ring, b) + (c * kGemmRows + row) * 4;
-          a0 += load_cluster(at);
-          a1 += load_cluster(at + kGemmRows * 4);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int4 u = load_shared(from + b * kGroup + i * kQuad);
+            v[4 * i] += u.x, v[4 * i + 1] += u.y, v[4 * i + 2] += u.z, v[4 * i + 3] += u.w;
+          }
         }
-        finish_pair<ACT, BF16>(p, f, m0 + c, a0, a1, x_scale[c], x_scale[c + 1]);
+        finish16<ACT, BF16>(p, f, m0 + 16 * g, p.M - m0 - 16 * g, v, sh.x_scale + 16 * g);
       }
     }
-    cluster_sync();  // no block ends while another may still read its sums
   } else {
+    tmem_fence_before();
     __syncwarp();
     __syncthreads();
   }
@@ -228,6 +236,7 @@ static mgv_status encode_rows(CUtensorMap *map, const void *ptr, int64_t rows, i
 // columns / 8 at bit 17, rows / 16 at bit 24.
 static uint32_t instruction(int rows, int columns) { return 2u << 4 | 1u << 7 | 1u << 10 | uint32_t(columns / 8) << 17 | uint32_t(rows / 16) << 24; }
 
+// bt, split: 0 where the plan is free to choose.
 static mgv_status plan_block(GemmI8Plan &pl, int64_t M, int bt, int split, int sms, int most) {
   GemmI8Params &p = pl.p;
   // columns of the matrix instruction: 16, or a multiple of 32 up to 256
@@ -237,24 +246,28 @@ static mgv_status plan_block(GemmI8Plan &pl, int64_t M, int bt, int split, int s
   const int slices = (p.K + kGemmK - 1) / kGemmK;
   p.split = 1;
   while (p.split < 8 && 2 * p.split <= slices && tiles * p.split < sms * 7 / 8) p.split *= 2;
-  if (split) p.split = std::min(1 << (split - 1), 8);
-  while (p.split > slices) p.split /= 2;
+  if (split) p.split = split;
+  p.split = std::min(p.split, slices);
   const int64_t grid = tiles * p.split;
   if (grid > 0x7fffffff) return fail(MGV_STATUS_UNSUPPORTED, "gemm_i8: too many tiles (M=%lld N=%d)", (long long)M, p.N);
   pl.grid = int(grid);
   pl.cluster = p.split;
   p.tmem_cols = 32;
   while (int(p.tmem_cols) < p.bt) p.tmem_cols *= 2;
-  const int slot = kGemmABytes + p.bt * kGemmK, room = most - 4096;  // static shared memory and alignment
-  const int share = (slices + p.split - 1) / p.split;
-  p.stages = std::min(std::min(share, kGemmMaxStages), (grid > sms ? room / 2 : room) / slot);
-  p.stages = std::max(p.stages, std::min(2, share));
-  // the sums of a split tile need bt x 128 words; and blocks that fit an SM by their shared memory must fit
-  // it by their tensor memory too (512 columns), or one would wait in its allocation for another to end
+  // Shared memory of a block: its share of an SM by the number of blocks an SM gets.  Blocks that fit an SM by
+  // their shared memory must fit it by their tensor memory too (512 columns), or one would wait in its
+  // allocation for another to end: at least the same fraction of both.
+  const int slot = kGemmABytes + p.bt * kGemmK, share = (slices + p.split - 1) / p.split;
+  const int fixed = kGemmReserved + int(sizeof(GemmBlockShared));  // beside the dynamic part; kGemmAlign of that goes to alignment
+  const int64_t wanted = std::min<int64_t>((grid + sms - 1) / sms, 512 / p.tmem_cols);
+  int per_sm = int(std::max<int64_t>(1, wanted));
+  while (per_sm > 1 && (kGemmSmShared / per_sm - fixed - kGemmAlign) / slot < std::min(3, share)) --per_sm;
+  const int room = std::min(kGemmSmShared / per_sm - fixed, most - int(sizeof(GemmBlockShared))) - kGemmAlign;
+  p.stages = std::min(std::min(share, kGemmMaxStages), room / slot);
   int smem = p.stages * slot;
-  if (p.split > 1) smem = std::max(smem, p.bt * kGemmRows * 4);
-  smem = std::max(smem, int(int64_t(most) * p.tmem_cols / 512));
-  pl.smem = std::min(smem + 1024, room + 1024);
+  if (p.split > 1) smem = std::max(smem, (p.bt / 16 + p.split - 1) / p.split * p.split * kGemmRows * 64);  // the sums of a split tile
+  smem = std::max(smem + kGemmAlign, int(int64_t(kGemmSmShared) * p.tmem_cols / 512) - fixed);
+  pl.smem = smem;
   p.idesc = instruction(kGemmRows, p.bt);
   return MGV_STATUS_OK;
 }
@@ -270,9 +283,9 @@ static void plan_pair(GemmI8Plan &pl, int64_t M, int bt, int sms, int most) {
   pl.cluster = 2;
   p.tmem_cols = 64;  // two accumulators
   while (int(p.tmem_cols) < 2 * p.bt) p.tmem_cols *= 2;
-  const int slot = kGemmABytes + p.bt / 2 * kGemmK, room = most - 4096;
-  p.stages = std::min(kGemmMaxStages, room / slot);
-  pl.smem = room + 1024;  // one block per SM: it may hold all of the tensor memory
+  const int slot = kGemmABytes + p.bt / 2 * kGemmK, room = most - int(sizeof(GemmPairShared));
+  p.stages = std::min(kGemmMaxStages, (room - kGemmAlign) / slot);
+  pl.smem = room;  // one block per SM: it may hold all of the tensor memory
   p.idesc = instruction(2 * kGemmRows, p.bt);
 }
 
@@ -299,7 +312,7 @@ static mgv_status prepare(const mgv_gemm_i8_args *a, mgv_gemm_i8_plan &pl) {
   const int want = (a->hints >> 8) & 31;
   pl.pair = a->hints & MGV_GEMM_HINT_PAIR || (!(a->hints & MGV_GEMM_HINT_BLOCK) && a->M > 256);
   if (pl.pair) plan_pair(pl, a->M, want ? std::min(256, (want + 1) / 2 * 32) : 0, sms, most);
-  else if ((st = plan_block(pl, a->M, want == 1 ? 16 : std::min(256, (want + 1) / 2 * 32), a->hints & 7, sms, most)) != MGV_STATUS_OK) return st;
+  else if ((st = plan_block(pl, a->M, want == 1 ? 16 : std::min(256, (want + 1) / 2 * 32), want ? (a->hints & 7) + 1 : 0, sms, most)) != MGV_STATUS_OK) return st;
   if ((st = encode_rows(&p.w_map, a->weights, a->N, a->K, a->ldw, kGemmRows)) != MGV_STATUS_OK) return st;
   return encode_rows(&p.x_map, a->x, a->M, a->K, a->ldx, pl.pair ? p.bt / 2 : p.bt);
 }

@@ -23,22 +23,21 @@ __device__ __forceinline__ TileAt tile_at(const GemmI8Params &p, uint32_t tile) 
 template <int ACT, bool BF16>
 __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_pair_kernel(const __grid_constant__ GemmI8Params p) {
   extern __shared__ uint8_t dynamic[];
-  __shared__ alignas(8) uint64_t full[kGemmMaxStages], empty[kGemmMaxStages], ready[2], drained[2];
-  __shared__ uint32_t tmem_base;
+  __shared__ GemmPairShared sh;
   const uint32_t ring = (smem_u32(dynamic) + 1023) & ~1023u;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const uint32_t rank = cluster_rank();
   const uint32_t pairs = gridDim.x / 2, pair = blockIdx.x / 2, tiles = uint32_t(p.n_tiles) * uint32_t(p.m_tiles);
   const int slices = (p.K + kGemmK - 1) / kGemmK;
   const uint32_t slot_bytes = kGemmABytes + p.bt / 2 * kGemmK;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < p.stages; ++i) bar_init(smem_u32(&full[i]), 1), bar_init(smem_u32(&empty[i]), 1);
-    for (int i = 0; i < 2; ++i) bar_init(smem_u32(&ready[i]), 1), bar_init(smem_u32(&drained[i]), 8);
+    for (int i = 0; i < p.stages; ++i) bar_init(smem_u32(&sh.full[i]), 1), bar_init(smem_u32(&sh.empty[i]), 1);
+    for (int i = 0; i < 2; ++i) bar_init(smem_u32(&sh.ready[i]), 1), bar_init(smem_u32(&sh.drained[i]), 8);
     asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(p.tmem_cols) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(p.tmem_cols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
   }
   tmem_fence_before();
@@ -46,94 +45,103 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_pair_kernel(const __g
   __syncthreads();
   cluster_sync();
   tmem_fence_after();
-  const uint32_t tmem = tmem_base;
+  const uint32_t tmem = __shfl_sync(~0u, sh.tmem_base, 0);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {
     // both blocks' copies count on the first block's barriers; each block waits on its own for a free slot
+    const bool one = elect_one();
     TileAt at = tile_at(p, pair);
     const int ahead = min(slices, p.stages);
-    for (int i = 0; i < ahead; ++i) {
-      if (rank == 0) bar_expect(smem_u32(&full[i]), 2 * slot_bytes);
-      box_load_pair(ring + i * slot_bytes, &p.w_map, i * kGemmK, at.n0 + int(rank) * kGemmRows, in_block(smem_u32(&full[i]), 0));
+    if (one) {
+      for (int i = 0; i < ahead; ++i) {
+        if (rank == 0) bar_expect(smem_u32(&sh.full[i]), 2 * slot_bytes);
+        box_load_pair(ring + i * slot_bytes, &p.w_map, i * kGemmK, at.n0 + int(rank) * kGemmRows, in_block(smem_u32(&sh.full[i]), 0));
+      }
     }
     asm volatile("griddepcontrol.wait;\n\tfence.proxy.async.global;" ::: "memory");
-    for (int i = 0; i < ahead; ++i)
-      box_load_pair(ring + i * slot_bytes + kGemmABytes, &p.x_map, i * kGemmK, at.m0 + int(rank) * p.bt / 2, in_block(smem_u32(&full[i]), 0));
+    if (one)
+      for (int i = 0; i < ahead; ++i)
+        box_load_pair(ring + i * slot_bytes + kGemmABytes, &p.x_map, i * kGemmK, at.m0 + int(rank) * p.bt / 2, in_block(smem_u32(&sh.full[i]), 0));
     int slot = ahead % p.stages;
     uint32_t issued = ahead, phase = 0;  // phase: of `empty` once the ring is full
     bool ok = true;
     for (uint32_t tile = pair; tile < tiles && ok; tile += pairs) {
       at = tile_at(p, tile);
       for (int i = tile == pair ? ahead : 0; i < slices; ++i) {
-        if (issued >= uint32_t(p.stages) && !(ok = bar_wait(smem_u32(&empty[slot]), phase, p.err))) break;
-        const uint32_t bar = in_block(smem_u32(&full[slot]), 0), dst = ring + slot * slot_bytes;
-        if (rank == 0) bar_expect(smem_u32(&full[slot]), 2 * slot_bytes);
-        box_load_pair(dst, &p.w_map, i * kGemmK, at.n0 + int(rank) * kGemmRows, bar);
-        box_load_pair(dst + kGemmABytes, &p.x_map, i * kGemmK, at.m0 + int(rank) * p.bt / 2, bar);
-        if (issued >= uint32_t(p.stages) && slot == p.stages - 1) phase ^= 1;
+        if (issued >= uint32_t(p.stages)) {
+          ok = bar_wait(smem_u32(&sh.empty[slot]), phase, p.err);
+          if (!ok) break;
+          if (slot == p.stages - 1) phase ^= 1;
+        }
+        if (one) {
+          const uint32_t bar = in_block(smem_u32(&sh.full[slot]), 0), dst = ring + slot * slot_bytes;
+          if (rank == 0) bar_expect(smem_u32(&sh.full[slot]), 2 * slot_bytes);
+          box_load_pair(dst, &p.w_map, i * kGemmK, at.n0 + int(rank) * kGemmRows, bar);
+          box_load_pair(dst + kGemmABytes, &p.x_map, i * kGemmK, at.m0 + int(rank) * p.bt / 2, bar);
+        }
         if (++slot == p.stages) slot = 0;
         ++issued;
       }
     }
     // The blocks end only when their slots have been read (and so filled): every slot's last release is
-    // waited for.  If the matrix thread gave up, the first block waits for the copies of both instead.
+    // waited for.  If the matrix warp gave up, the first block waits for the copies of both instead.
     for (uint32_t i = issued > uint32_t(p.stages) ? issued - p.stages : 0; i < issued && ok; ++i)
-      ok = bar_wait(smem_u32(&empty[i % p.stages]), (i / p.stages) & 1, p.err);
+      ok = bar_wait(smem_u32(&sh.empty[i % p.stages]), (i / p.stages) & 1, p.err);
     if (!ok && rank == 0)
       for (uint32_t i = issued > uint32_t(p.stages) ? issued - p.stages : 0; i < issued; ++i)
-        if (!bar_wait(smem_u32(&full[i % p.stages]), (i / p.stages) & 1, p.err)) break;
-  } else if (warp == 1 && lane == 0 && rank == 0) {
+        if (!bar_wait(smem_u32(&sh.full[i % p.stages]), (i / p.stages) & 1, p.err)) break;
+  } else if (warp == 1 && rank == 0) {
+    const bool one = elect_one();
     int slot = 0;
     uint32_t phase = 0, turn = 0;
     bool ok = true;
     for (uint32_t tile = pair; tile < tiles && ok; tile += pairs, ++turn) {
       const uint32_t buf = turn & 1, acc = tmem + buf * (p.tmem_cols / 2);
-      if (turn >= 2 && !(ok = bar_wait(smem_u32(&drained[buf]), ((turn >> 1) - 1) & 1, p.err))) break;
+      if (turn >= 2) ok = bar_wait<true>(smem_u32(&sh.drained[buf]), ((turn >> 1) - 1) & 1, p.err);
       tmem_fence_after();
-      for (int i = 0; i < slices; ++i) {
-        if (!(ok = bar_wait(smem_u32(&full[slot]), phase, p.err))) break;
+      for (int i = 0; i < slices && ok; ++i) {
+        ok = bar_wait(smem_u32(&sh.full[slot]), phase, p.err);
+        if (!ok) break;
         tmem_fence_after();
         const uint64_t a = operand_desc(ring + slot * slot_bytes), b = operand_desc(ring + slot * slot_bytes + kGemmABytes);
+        if (one) {
 #pragma unroll
-        for (int k = 0; k < kGemmK / 32; ++k) {
-          const uint32_t add = i + k > 0;
-          asm volatile(
-              "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %4, 0;\n\t"
-              "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, q;\n\t}" ::"r"(acc),
-              "l"(a + 2 * k), "l"(b + 2 * k), "r"(p.idesc), "r"(add)
-              : "memory");
+          for (int k = 0; k < kGemmK / 32; ++k) multiply_add<2>(acc, a + 2 * k, b + 2 * k, p.idesc, i + k > 0);
+          commit_pair(smem_u32(&sh.empty[slot]));
         }
-        commit_pair(smem_u32(&empty[slot]));
+        __syncwarp();
         if (++slot == p.stages) slot = 0, phase ^= 1;
       }
-      if (ok) commit_pair(smem_u32(&ready[buf]));
+      if (ok && one) commit_pair(smem_u32(&sh.ready[buf]));
+      __syncwarp();
     }
   } else if (warp >= 2) {
     const int quarter = warp % 4, row = int(rank) * kGemmRows + quarter * 32 + lane;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     uint32_t turn = 0;
+    bool good = true;
     for (uint32_t tile = pair; tile < tiles; tile += pairs, ++turn) {
       const TileAt at = tile_at(p, tile);
       const uint32_t buf = turn & 1, lanes = tmem + buf * (p.tmem_cols / 2) + (uint32_t(quarter * 32) << 16);
       const Feature f = load_feature<BF16>(p, at.n0 + row);
-      if (!__all_sync(~0u, bar_wait(smem_u32(&ready[buf]), (turn >> 1) & 1, p.err))) break;
+      // the buffer's last readers have passed the barrier of the tile between
+      for (int i = threadIdx.x - 64; i < p.bt; i += 128) sh.x_scale[buf][i] = at.m0 + i < p.M ? p.x_scale[at.m0 + i] : 0.0f;
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      good = good && bar_wait(smem_u32(&sh.ready[buf]), (turn >> 1) & 1, p.err);
+      if (!good) continue;  // on to the barrier that the other warps wait at
       tmem_fence_after();
       const int columns = min(p.bt, p.M - at.m0);
       for (int c = 0; c < columns; c += 16) {
         int v[16];
         __syncwarp();
         tmem_load16(lanes + c, v);
-        const int mine = at.m0 + c + (lane & 15);
-        const float scales = mine < p.M ? p.x_scale[mine] : 0.0f;
         tmem_wait_load();
-#pragma unroll
-        for (int i = 0; i < 16; i += 2)
-          finish_pair<ACT, BF16>(p, f, at.m0 + c + i, v[i], v[i + 1], __shfl_sync(~0u, scales, i), __shfl_sync(~0u, scales, i + 1));
+        finish16<ACT, BF16>(p, f, at.m0 + c, columns - c, v, sh.x_scale[buf] + c);
       }
       tmem_fence_before();
       __syncwarp();
-      if (lane == 0) arrive_in_block(in_block(smem_u32(&drained[buf]), 0));
+      if (lane == 0) arrive_in_block(in_block(smem_u32(&sh.drained[buf]), 0));
     }
   }
   __syncwarp();

@@ -34,7 +34,23 @@ constexpr int kGemmK = 128;                // K of a ring slot: one 128-byte swi
 constexpr int kGemmABytes = kGemmRows * kGemmK;
 constexpr int kGemmThreads = 192;          // producer warp, matrix warp, four epilogue warps
 constexpr int kGemmMaxStages = 16;
+constexpr int kGemmAlign = 1024;           // of the ring; dynamic shared memory lost to it at most
+constexpr int kGemmReserved = 1024;        // shared memory the system takes for each block
+constexpr int kGemmSmShared = 228 * 1024;  // of an SM
 constexpr int kGemmTimeout = 0x100;        // bit of the device error word
+
+// Static shared memory of the two kernels.
+struct GemmBlockShared {
+  alignas(16) float x_scale[256];
+  uint64_t full[kGemmMaxStages], empty[kGemmMaxStages], done;
+  uint32_t tmem_base;
+  int failed;
+};
+struct GemmPairShared {
+  alignas(16) float x_scale[2][256];
+  uint64_t full[kGemmMaxStages], empty[kGemmMaxStages], ready[2], drained[2];
+  uint32_t tmem_base;
+};
 
 enum { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGated = 3 };
 
@@ -46,26 +62,45 @@ __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+// One lane of a converged warp.  The roles below are whole warps with one lane elected for the
+// instructions that a single thread issues: with operands and control flow the same for the warp, a
+// matrix instruction takes 40 cycles to issue and a slot's wait, four instructions and commit 265;
+// the same by a lone thread in a branch of its own, with waits of cluster scope, took 640.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.b32 %0, 1, 0, q;\n\t}" : "=r"(one));
+  return one;
+}
+template <bool CLUSTER>
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
-  asm volatile("{\n\t.reg .pred q;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 q, [%1], %2;\n\tselp.b32 %0, 1, 0, q;\n\t}"
-               : "=r"(ok)
-               : "r"(bar), "r"(parity)
-               : "memory");
+  if (CLUSTER)
+    asm volatile("{\n\t.reg .pred q;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 q, [%1], %2;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+                 : "=r"(ok)
+                 : "r"(bar), "r"(parity)
+                 : "memory");
+  else
+    asm volatile("{\n\t.reg .pred q;\n\tmbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+                 : "=r"(ok)
+                 : "r"(bar), "r"(parity)
+                 : "memory");
   return ok;
 }
-// Waits for the phase of the given parity, for at most about a second; false (and the device error
-// word set) when it gave up.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, int *err) {
-  for (int i = 0; i < 1024; ++i)
-    if (bar_try(bar, parity)) return true;
+template <bool CLUSTER>
+__device__ __noinline__ bool bar_wait_long(uint32_t bar, uint32_t parity, int *err) {
+  bool ok = false;
+  for (int i = 0; i < 1024 && !ok; ++i) ok = bar_try<CLUSTER>(bar, parity);
   const uint64_t t0 = global_timer_ns();
-  do {
-    for (int i = 0; i < 256; ++i)
-      if (bar_try(bar, parity)) return true;
-  } while (global_timer_ns() - t0 < 1000000000ull);
-  atomicOr(err, kGemmTimeout);
-  return false;
+  while (!ok && global_timer_ns() - t0 < 1000000000ull)
+    for (int i = 0; i < 256 && !ok; ++i) ok = bar_try<CLUSTER>(bar, parity);
+  if (!ok) atomicOr(err, kGemmTimeout);
+  return __all_sync(~0u, ok);
+}
+// A warp waits for the phase of the given parity, for at most about a second; false, for all its lanes
+// and with the device error word set, when it gave up.  CLUSTER: threads of another block arrive here.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, int *err) {
+  return __all_sync(~0u, bar_try<CLUSTER>(bar, parity)) || bar_wait_long<CLUSTER>(bar, parity, err);
 }
 
 // One box of a tensor map into shared memory of this block; bytes are counted on bar.
@@ -87,6 +122,21 @@ __device__ __forceinline__ void box_load_pair(uint32_t dst, const CUtensorMap *m
 // eight rows 1024 bytes apart.
 __device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
   return (uint64_t(addr & 0x3ffff) >> 4) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+
+// D (tensor memory) = or += A (rows x 32) * B (columns x 32)^T of int8 operands, by one SM or a pair
+template <int SMS>
+__device__ __forceinline__ void multiply_add(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  if (SMS == 1)
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, q;\n\t}" ::"r"(d), "l"(a),
+        "l"(b), "r"(idesc), "r"(add)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, q;\n\t}" ::"r"(d), "l"(a),
+        "l"(b), "r"(idesc), "r"(add)
+        : "memory");
 }
 
 // 16 accumulator columns of the warp's 32 lanes.
@@ -125,9 +175,13 @@ __device__ __forceinline__ void commit_pair(uint32_t bar) {
                "h"(uint16_t(3))
                : "memory");
 }
-__device__ __forceinline__ int load_cluster(uint32_t addr) {
-  int v;
-  asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+// 16 bytes into the shared memory of a block of the cluster, and out of the own one
+__device__ __forceinline__ void store_cluster(uint32_t addr, int a, int b, int c, int d) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ int4 load_shared(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
 }
 
@@ -161,35 +215,58 @@ __device__ __forceinline__ Feature load_feature(const GemmI8Params &p, int n) {
   return f;
 }
 
-// Sums of two neighbouring rows m, m + 1 of the activations for the lane's feature, scaled,
-// activated and stored.  Lanes 2i and 2i + 1 swap one value each, so that the even lane holds both
-// features of row m and the odd lane both of row m + 1: one 32-bit store, or gate and up together.
-// All 32 lanes call it.
+// Sums of 16 neighbouring activation rows from m on for the lane's feature -- `rows` of them exist --
+// scaled, activated and stored.  Lanes 2i and 2i + 1 swap half of their values, so that the even
+// lane holds both features of the even rows and the odd lane both of the odd rows: one 32-bit store for two
+// features, or gate and up together.  All 32 lanes call it; x_scale is 16-byte aligned.
 template <int ACT, bool BF16>
-__device__ __forceinline__ void finish_pair(const GemmI8Params &p, const Feature &f, int m, int a0, int a1, float s0, float s1) {
-  float v0 = fmaf(float(a0), f.scale * s0, f.bias), v1 = fmaf(float(a1), f.scale * s1, f.bias);
-  if (ACT == kActRelu) v0 = v0 < 0.0f ? 0.0f : v0, v1 = v1 < 0.0f ? 0.0f : v1;
-  if (ACT == kActSilu) v0 = silu(v0), v1 = silu(v1);
-  const bool odd = f.n & 1;
+__device__ __forceinline__ void finish16(const GemmI8Params &p, const Feature &f, int m, int rows, const int (&v)[16], const float *x_scale) {
+  float y[16];
+#pragma unroll
+  for (int i = 0; i < 16; i += 4) {
+    const float4 s = *reinterpret_cast<const float4 *>(x_scale + i);
+    y[i] = fmaf(float(v[i]), f.scale * s.x, f.bias);
+    y[i + 1] = fmaf(float(v[i + 1]), f.scale * s.y, f.bias);
+    y[i + 2] = fmaf(float(v[i + 2]), f.scale * s.z, f.bias);
+    y[i + 3] = fmaf(float(v[i + 3]), f.scale * s.w, f.bias);
+  }
+  if (ACT == kActRelu || ACT == kActSilu) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) y[i] = ACT == kActSilu ? silu(y[i]) : y[i] < 0.0f ? 0.0f : y[i];
+  }
+  const int odd = f.n & 1;
   uint16_t *out = static_cast<uint16_t *>(p.out);
   if (ACT == kActGated || p.wide) {
-    const float got = __shfl_xor_sync(~0u, odd ? v0 : v1, 1);
-    const float lo = odd ? got : v0, hi = odd ? v1 : got;
-    const int row = m + (odd ? 1 : 0);
-    if (row >= p.M) return;
+    float got[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) got[i] = __shfl_xor_sync(~0u, odd ? y[2 * i] : y[2 * i + 1], 1);
     if (ACT == kActGated) {
-      if (f.inside) out[int64_t(row) * p.ldd + (f.n >> 1)] = round_out<BF16>(silu(lo) * hi);
-      return;
+      uint16_t *at = out + int64_t(m + odd) * p.ldd + (f.n >> 1);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float gate = odd ? got[i] : y[2 * i], up = odd ? y[2 * i + 1] : got[i];
+        if (f.inside && 2 * i + odd < rows) *at = round_out<BF16>(silu(gate) * up);
+        at += 2 * p.ldd;
+      }
+    } else {
+      const bool both = (f.n | 1) < p.N, one = !both && (f.n & ~1) < p.N;  // the last feature of an odd N stands alone
+      uint16_t *at = out + int64_t(m + odd) * p.ldd + (f.n & ~1);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t lo = round_out<BF16>(odd ? got[i] : y[2 * i]), hi = round_out<BF16>(odd ? y[2 * i + 1] : got[i]);
+        if (both && 2 * i + odd < rows) *reinterpret_cast<uint32_t *>(at) = lo | hi << 16;
+        if (one && 2 * i + odd < rows) *at = uint16_t(lo);
+        at += 2 * p.ldd;
+      }
     }
-    const int n = f.n & ~1;
-    uint16_t *at = out + int64_t(row) * p.ldd + n;
-    if (n + 1 < p.N) *reinterpret_cast<uint32_t *>(at) = uint32_t(round_out<BF16>(lo)) | uint32_t(round_out<BF16>(hi)) << 16;
-    else if (n < p.N) *at = round_out<BF16>(lo);
     return;
   }
-  if (!f.inside) return;
-  if (m < p.M) out[int64_t(m) * p.ldd + f.n] = round_out<BF16>(v0);
-  if (m + 1 < p.M) out[int64_t(m + 1) * p.ldd + f.n] = round_out<BF16>(v1);
+  uint16_t *at = out + int64_t(m) * p.ldd + f.n;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    if (f.inside && i < rows) *at = round_out<BF16>(y[i]);
+    at += p.ldd;
+  }
 }
 
 #endif  // __CUDACC__
