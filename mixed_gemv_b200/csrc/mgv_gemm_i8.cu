@@ -12,8 +12,10 @@ namespace mgv {
 // column operand, whose width goes from 16 up: one token costs a sixteen-column tile, not 128 rows.
 // Weights and activations reach a ring of shared-memory slots by tiled bulk copies, one thread issues
 // the matrix instructions, accumulators are 32-bit integers in tensor memory: lane = feature, column =
-// row of the activations.  With split > 1 every block sends each other one its sums of that block's share of the columns, and
-// adds and finishes its own share; integer sums, so the result does not depend on the split.
+// row of the activations.  With split > 1 every block finishes a share of the columns, out of the sums that all
+// blocks of the cluster send it; integer sums, so the result does not depend on the split.
+constexpr int kQuadBytes = kGemmRows * 16;  // sums of 128 features x 4 columns
+
 template <int ACT, bool BF16>
 __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_block_kernel(const __grid_constant__ GemmI8Params p) {
   extern __shared__ uint8_t dynamic[];
@@ -27,37 +29,42 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_block_kernel(const __
   const int first = int(int64_t(slices) * rank / p.split), count = int(int64_t(slices) * (rank + 1) / p.split) - first;
   const uint32_t slot_bytes = kGemmABytes + p.bt * kGemmK;
 
-  if (threadIdx.x == 0) {
+  const bool one = elect_one();
+  const int ahead = min(count, p.stages);  // slots of the first ring fill
+  if (warp == 0 && one) {
     for (int i = 0; i < p.stages; ++i) bar_init(smem_u32(&sh.full[i]), 1), bar_init(smem_u32(&sh.empty[i]), 1);
     bar_init(smem_u32(&sh.done), 1);
+    bar_init(smem_u32(&sh.sums), 1);
     sh.failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async;" ::: "memory");
+    // the weights first of all: before the rest of the set-up, and before the wait for the previous kernel
+    for (int i = 0; i < ahead; ++i) {
+      bar_expect(smem_u32(&sh.full[i]), slot_bytes);
+      box_load(ring + i * slot_bytes, &p.w_map, (first + i) * kGemmK, n0, smem_u32(&sh.full[i]));
+    }
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(p.tmem_cols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   tmem_fence_before();
+  __syncwarp();
   __syncthreads();
   tmem_fence_after();
   const uint32_t tmem = __shfl_sync(~0u, sh.tmem_base, 0);
   // only now: a dependent kernel that starts on this SM may hold tensor memory while it waits for this one to end
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int columns = min(p.bt, p.M - m0), quads = (columns + 3) / 4;
+  const int mine = p.split > 1 ? (quads - int(rank) + p.split - 1) / p.split : 0;  // column quads this block finishes of a split tile
+  if (p.split > 1 && p.sums_off) cluster_arrive<true>();  // this block can be sent to: its barriers are set up
 
   if (warp == 0) {
-    // weights of the first ring fill before the wait for the previous kernel, its output (x) after it
-    const bool one = elect_one();
-    const int ahead = min(count, p.stages);
-    if (one) {
-      for (int i = 0; i < ahead; ++i) {
-        bar_expect(smem_u32(&sh.full[i]), slot_bytes);
-        box_load(ring + i * slot_bytes, &p.w_map, (first + i) * kGemmK, n0, smem_u32(&sh.full[i]));
-      }
-    }
     asm volatile("griddepcontrol.wait;\n\tfence.proxy.async.global;" ::: "memory");
-    if (one)
+    if (one) {
       for (int i = 0; i < ahead; ++i)
         box_load(ring + i * slot_bytes + kGemmABytes, &p.x_map, (first + i) * kGemmK, m0, smem_u32(&sh.full[i]));
+      if (mine > 0) bar_expect(smem_u32(&sh.sums), mine * p.split * kQuadBytes);
+    }
     int slot = 0, issued = ahead;
     uint32_t phase = 0;
     for (int i = ahead; i < count; ++i, ++issued) {
@@ -74,7 +81,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_block_kernel(const __
     for (int i = max(0, issued - p.stages); i < issued; ++i)
       if (!bar_wait(smem_u32(&sh.full[i % p.stages]), (i / p.stages) & 1, p.err)) break;
   } else if (warp == 1) {
-    const bool one = elect_one();
     int slot = 0;
     uint32_t phase = 0;
     bool ok = true;
@@ -99,62 +105,71 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_block_kernel(const __
   }
 
   // tensor memory: a warp reads the 32 lanes of its number modulo 4
-  const int quarter = warp % 4, row = quarter * 32 + lane;
+  const int quarter = warp % 4, half = warp >= 6, row = quarter * 32 + lane;
   const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
   bool good = true;
   Feature f = {};
   if (warp >= 2) {
     f = load_feature<BF16>(p, n0 + row);
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    for (int i = threadIdx.x - 64; i < p.bt; i += 128) sh.x_scale[i] = m0 + i < p.M ? p.x_scale[m0 + i] : 0.0f;
-    asm volatile("bar.sync 1, 128;" ::: "memory");
+    if (const int i = threadIdx.x - 64; i < p.bt) sh.x_scale[i] = m0 + i < p.M ? p.x_scale[m0 + i] : 0.0f;
+    asm volatile("bar.sync 1, %0;" ::"n"(kGemmEpilogue) : "memory");
     good = bar_wait(smem_u32(&sh.done), 0, p.err) && !*static_cast<volatile int *>(&sh.failed);
     tmem_fence_after();
     if (p.split == 1 && good) {
-      const int columns = min(p.bt, p.M - m0);
-      for (int c = 0; c < columns; c += 16) {
+      for (int c = half * 16; c < columns; c += 32) {
         int v[16];
         __syncwarp();
         tmem_load16(lanes + c, v);
         tmem_wait_load();
-        finish16<ACT, BF16>(p, f, m0 + c, columns - c, v, sh.x_scale + c);
+        finish<ACT, BF16>(p, f, m0 + c, columns - c, v, sh.x_scale + c);
       }
     }
   }
   if (p.split > 1) {
-    // Every copy of the cluster has landed and every matrix instruction has read its slot: the rings'
-    // memory is free for the sums.  Block r finishes the 16-column groups r, r + split, ...; of each it
-    // gets, from each block, [4 quads of columns][128 features][4 columns].
-    cluster_sync();
-    const int groups = (min(p.bt, p.M - m0) + 15) / 16;
-    constexpr int kQuad = kGemmRows * 16, kGroup = 4 * kQuad;
+    // Block r finishes the column quads r, r + split, ...; of each it gets [128 features][4 columns] from
+    // every block, itself among them.  Where that goes into the ring, every copy of the cluster has to have
+    // landed and every matrix instruction to have read its slot.
+    if (!p.sums_off) cluster_arrive<true>();
+    cluster_wait();
+    const uint32_t sums = p.sums_off ? smem_u32(dynamic) + p.sums_off : ring;
     if (warp >= 2) {
-      for (int g = 0; g < groups; ++g) {
+      for (int c = half * 16; c < columns && good; c += 32) {
         int v[16];
         __syncwarp();
-        tmem_load16(lanes + 16 * g, v);
+        tmem_load16(lanes + c, v);
         tmem_wait_load();
-        const uint32_t to = in_block(ring, g % p.split) + ((g / p.split) * p.split + rank) * kGroup + row * 16;
+        int owner = c / 4 % p.split, at = c / 4 - owner + int(rank);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) store_cluster(to + i * kQuad, v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        for (int i = 0; i < 4; ++i) {
+          if (c / 4 + i < quads)
+            send16(in_block(sums + at * kQuadBytes + row * 16, owner), in_block(smem_u32(&sh.sums), owner), v[4 * i], v[4 * i + 1],
+                   v[4 * i + 2], v[4 * i + 3]);
+          if (++owner == p.split) owner = 0, at += p.split;
+        }
       }
       tmem_fence_before();
     }
-    cluster_sync();
-    if (warp >= 2 && good) {
-      for (int g = int(rank); g < groups; g += p.split) {
-        const uint32_t from = ring + (g / p.split) * p.split * kGroup + row * 16;
-        int v[16] = {};
-        for (int b = 0; b < p.split; ++b) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int4 u = load_shared(from + b * kGroup + i * kQuad);
-            v[4 * i] += u.x, v[4 * i + 1] += u.y, v[4 * i + 2] += u.z, v[4 * i + 3] += u.w;
+    cluster_arrive<false>();
+    // Only blocks that finish columns are sent anything, and they wait for all of it: after that none of
+    // them is written to.  Where the wait gave up, the block stays until all others have sent what they will.
+    if (mine > 0) {
+      if (!bar_wait<true>(smem_u32(&sh.sums), 0, p.err)) {
+        cluster_wait();
+      } else if (warp >= 2 && good) {
+        for (int quad = int(rank) + half * p.split; quad < quads; quad += 2 * p.split) {
+          const uint32_t from = sums + quad / p.split * p.split * kQuadBytes + row * 16;
+          int v[4] = {};
+          for (int b = 0; b < p.split; ++b) {
+            const int4 u = load_shared(from + b * kQuadBytes);
+            v[0] += u.x, v[1] += u.y, v[2] += u.z, v[3] += u.w;
           }
+          finish<ACT, BF16>(p, f, m0 + 4 * quad, columns - 4 * quad, v, sh.x_scale + 4 * quad);
         }
-        finish16<ACT, BF16>(p, f, m0 + 16 * g, p.M - m0 - 16 * g, v, sh.x_scale + 16 * g);
       }
     }
+    __syncwarp();
+    __syncthreads();
   } else {
     tmem_fence_before();
     __syncwarp();
@@ -236,57 +251,121 @@ static mgv_status encode_rows(CUtensorMap *map, const void *ptr, int64_t rows, i
 // columns / 8 at bit 17, rows / 16 at bit 24.
 static uint32_t instruction(int rows, int columns) { return 2u << 4 | 1u << 7 | 1u << 10 | uint32_t(columns / 8) << 17 | uint32_t(rows / 16) << 24; }
 
-// bt, split: 0 where the plan is free to choose.
-static mgv_status plan_block(GemmI8Plan &pl, int64_t M, int bt, int split, int sms, int most) {
+// The estimate that tilings are compared by, in cycles.  Measured on B200 (4096-deep reductions, 1.9 GHz): an
+// SM alone takes in 96 bytes a cycle from L2, all SMs together 7500 as single blocks and 9400 as pairs; a slice of
+// 128 K keeps the issuing warp for 330 cycles at least and the matrix unit for the time of its four
+// instructions; HBM delivers 3260 bytes a cycle but for the start and end of a block's row of slices; 16
+// columns of an epilogue take 320 cycles; a split tile's exchange takes 1500 and 45 a column beside the next call's
+// start.  (Of 19 shapes from 1 x 4096 x 4096 to 2048 x 8192 x 28672 -- rows x features x K -- the choice was within
+// 8 % of the best tiling on 17; on 64 x 12288 x 4096 and 131 x 4096 x 11008 it is 14 % off.)
+constexpr double kSmBytes = 96, kBlockBytes = 7500, kPairBytes = 9400, kHbmBytes = 3260, kIssue = 330, kColumn16 = 320, kStart = 4500;
+
+// chain: of the slices that one block works through; fed: to get all operands from L2 to the SMs
+static double estimate(double chain, double fed, double weights, double tail) {
+  return kStart + std::max(std::max(chain, fed), weights / kHbmBytes + 0.4 * chain) + tail;
+}
+
+static int rounded_columns(int want) { return want == 1 ? 16 : std::min(256, (want + 1) / 2 * 32); }
+
+static void plan_block(GemmI8Plan &pl, int64_t M, int bt, int split, int sms, int most) {
   GemmI8Params &p = pl.p;
-  // columns of the matrix instruction: 16, or a multiple of 32 up to 256
-  p.bt = bt ? bt : M <= 16 ? 16 : int(std::min<int64_t>(256, (M + 31) / 32 * 32));
+  p.bt = bt;
+  p.split = split;
   p.n_tiles = (p.N + kGemmRows - 1) / kGemmRows;
-  const int64_t tiles = p.n_tiles * ((M + p.bt - 1) / p.bt);
-  const int slices = (p.K + kGemmK - 1) / kGemmK;
-  p.split = 1;
-  while (p.split < 8 && 2 * p.split <= slices && tiles * p.split < sms * 7 / 8) p.split *= 2;
-  if (split) p.split = split;
-  p.split = std::min(p.split, slices);
-  const int64_t grid = tiles * p.split;
-  if (grid > 0x7fffffff) return fail(MGV_STATUS_UNSUPPORTED, "gemm_i8: too many tiles (M=%lld N=%d)", (long long)M, p.N);
-  pl.grid = int(grid);
-  pl.cluster = p.split;
+  p.m_tiles = int((M + bt - 1) / bt);
+  p.sums_off = 0;
   p.tmem_cols = 32;
-  while (int(p.tmem_cols) < p.bt) p.tmem_cols *= 2;
-  // Shared memory of a block: its share of an SM by the number of blocks an SM gets.  Blocks that fit an SM by
-  // their shared memory must fit it by their tensor memory too (512 columns), or one would wait in its
-  // allocation for another to end: at least the same fraction of both.
-  const int slot = kGemmABytes + p.bt * kGemmK, share = (slices + p.split - 1) / p.split;
+  while (int(p.tmem_cols) < bt) p.tmem_cols *= 2;
+  p.idesc = instruction(kGemmRows, bt);
+  const int64_t grid = int64_t(p.n_tiles) * p.m_tiles * split;
+  const int slices = (p.K + kGemmK - 1) / kGemmK, share = (slices + split - 1) / split, slot = kGemmABytes + bt * kGemmK;
+  // Shared memory of a block: its share of an SM by the number of blocks an SM gets, and half of it at most
+  // for narrow tiles, so that the next call's blocks can start fetching weights beside it.  Blocks that fit an
+  // SM by their shared memory must fit it by their tensor memory too (512 columns), or one would wait in
+  // its allocation for another to end: at least the same fraction of both.
   const int fixed = kGemmReserved + int(sizeof(GemmBlockShared));  // beside the dynamic part; kGemmAlign of that goes to alignment
-  const int64_t wanted = std::min<int64_t>((grid + sms - 1) / sms, 512 / p.tmem_cols);
-  int per_sm = int(std::max<int64_t>(1, wanted));
+  const int64_t on_sm = (grid + sms - 1) / sms;
+  int per_sm = int(std::max<int64_t>(bt <= 64 ? 2 : 1, std::min<int64_t>(on_sm, 512 / p.tmem_cols)));
   while (per_sm > 1 && (kGemmSmShared / per_sm - fixed - kGemmAlign) / slot < std::min(3, share)) --per_sm;
   const int room = std::min(kGemmSmShared / per_sm - fixed, most - int(sizeof(GemmBlockShared))) - kGemmAlign;
   p.stages = std::min(std::min(share, kGemmMaxStages), room / slot);
-  int smem = p.stages * slot;
-  if (p.split > 1) smem = std::max(smem, (p.bt / 16 + p.split - 1) / p.split * p.split * kGemmRows * 64);  // the sums of a split tile
-  smem = std::max(smem + kGemmAlign, int(int64_t(kGemmSmShared) * p.tmem_cols / 512) - fixed);
+  int smem = p.stages * slot + kGemmAlign;
+  if (split > 1) {  // the sums of a split tile: beside the ring where they fit, which saves a wait, else in it
+    const int sums = (bt / 4 + split - 1) / split * split * kQuadBytes;
+    if (smem + sums <= room + kGemmAlign) {
+      p.sums_off = smem;
+      smem += sums;
+    } else {
+      smem = std::max(smem, sums + kGemmAlign);
+    }
+  }
+  smem = std::max(smem, int(int64_t(kGemmSmShared) * p.tmem_cols / 512) - fixed);
+  pl.pair = 0;
   pl.smem = smem;
-  p.idesc = instruction(kGemmRows, p.bt);
-  return MGV_STATUS_OK;
+  pl.grid = int(std::min<int64_t>(grid, 0x7fffffff));
+  pl.cluster = split;
+  const int64_t at_once = std::max(1, std::min(kGemmSmShared / (smem + fixed), int(512 / p.tmem_cols)));
+  const double slice = std::max(slot / kSmBytes, 4 * std::max(40.0, bt / 2.0));  // of the SM's time
+  const double tail = split > 1 ? 1500 + 45.0 * bt : kColumn16 * ((bt + 15) / 16);
+  const int64_t rounds = (on_sm + at_once - 1) / at_once;  // blocks that follow one another: each starts and ends alone
+  const double chain = rounds * share * std::max(kIssue, slice) + (rounds - 1) * (2500 + tail);
+  const double fed = std::max(double(on_sm) * share * slice, double(grid) * share * slot / kBlockBytes);
+  pl.cost = estimate(chain, fed, double(p.N) * p.K, tail);
 }
 
 static void plan_pair(GemmI8Plan &pl, int64_t M, int bt, int sms, int most) {
   GemmI8Params &p = pl.p;
-  p.bt = bt ? bt : int(std::min<int64_t>(256, (M + 31) / 32 * 32));
-  p.n_tiles = (p.N + 2 * kGemmRows - 1) / (2 * kGemmRows);
-  p.m_tiles = int((M + p.bt - 1) / p.bt);
+  p.bt = bt;
   p.split = 1;
-  const int64_t tiles = int64_t(p.n_tiles) * p.m_tiles;
-  pl.grid = int(2 * std::min<int64_t>(tiles, sms / 2));
-  pl.cluster = 2;
+  p.n_tiles = (p.N + 2 * kGemmRows - 1) / (2 * kGemmRows);
+  p.m_tiles = int((M + bt - 1) / bt);
   p.tmem_cols = 64;  // two accumulators
-  while (int(p.tmem_cols) < 2 * p.bt) p.tmem_cols *= 2;
-  const int slot = kGemmABytes + p.bt / 2 * kGemmK, room = most - int(sizeof(GemmPairShared));
+  while (int(p.tmem_cols) < 2 * bt) p.tmem_cols *= 2;
+  p.idesc = instruction(2 * kGemmRows, bt);
+  const int64_t tiles = int64_t(p.n_tiles) * p.m_tiles, pairs = std::min<int64_t>(tiles, sms / 2);
+  const int slices = (p.K + kGemmK - 1) / kGemmK, slot = kGemmABytes + bt / 2 * kGemmK, room = most - int(sizeof(GemmPairShared));
   p.stages = std::min(kGemmMaxStages, (room - kGemmAlign) / slot);
+  pl.pair = 1;
   pl.smem = room;  // one block per SM: it may hold all of the tensor memory
-  p.idesc = instruction(2 * kGemmRows, p.bt);
+  pl.grid = int(2 * pairs);
+  pl.cluster = 2;
+  const double slice = std::max(std::max(slot / kSmBytes, kIssue), 2.0 * bt), tail = kColumn16 * (bt / 16);
+  const double chain = double((tiles + pairs - 1) / pairs) * std::max(slices * slice, tail);  // a tile's epilogue beside the next tile
+  pl.cost = estimate(chain, 2.0 * tiles * slices * slot / kPairBytes, double(p.N) * p.K, tail);
+}
+
+// The tiling of least estimated cost, of those that the hints leave.
+static mgv_status plan(GemmI8Plan &pl, const mgv_gemm_i8_args *a, int sms, int most) {
+  const int rows = (a->hints >> 8) & 31, slices = (a->K + kGemmK - 1) / kGemmK;
+  const int widest = int(std::min<int64_t>(256, (a->M + 31) / 32 * 32));
+  GemmI8Plan best;
+  best.cost = 0;
+  auto keep = [&](const GemmI8Plan &one) {
+    if (best.cost == 0 || one.cost < best.cost) best = one;
+  };
+  if (!(a->hints & MGV_GEMM_HINT_PAIR)) {
+    for (int bt = 16; bt <= 256; bt += bt == 16 ? 16 : 32) {
+      if (rows ? bt != rounded_columns(rows) : (a->M <= 16 ? bt > 16 : bt == 16 || bt > widest)) continue;
+      // clusters of 3, 5, 6 or 7 blocks leave SMs of a GPC empty: 131 x 12288 x 4096 in threes takes 20 us, in ones 13
+      for (int split = 1; split <= std::min(8, slices); split = rows ? split + 1 : 2 * split) {
+        if (rows && split != std::min((a->hints & 7) + 1, slices)) continue;
+        plan_block(pl, a->M, bt, split, sms, most);
+        keep(pl);
+      }
+    }
+  }
+  if (!(a->hints & MGV_GEMM_HINT_BLOCK)) {
+    for (int bt = 32; bt <= 256; bt += 32) {
+      if (rows ? bt != std::max(32, rounded_columns(rows)) : bt > widest) continue;
+      plan_pair(pl, a->M, bt, sms, most);
+      keep(pl);
+    }
+  }
+  if (best.cost == 0) return fail(MGV_STATUS_INVALID_ARGUMENT, "gemm_i8: hints %d leave no kernel", a->hints);
+  pl = best;
+  const int64_t blocks = int64_t(pl.p.n_tiles) * pl.p.m_tiles * pl.p.split;
+  if (blocks > 0x7fffffff) return fail(MGV_STATUS_UNSUPPORTED, "gemm_i8: too many tiles (M=%lld N=%d)", (long long)a->M, a->N);
+  return MGV_STATUS_OK;
 }
 
 static mgv_status prepare(const mgv_gemm_i8_args *a, mgv_gemm_i8_plan &pl) {
@@ -309,10 +388,7 @@ static mgv_status prepare(const mgv_gemm_i8_args *a, mgv_gemm_i8_plan &pl) {
   pl.act = a->flags & MGV_FLAG_ACT_RELU ? kActRelu : a->flags & MGV_FLAG_ACT_SILU ? kActSilu : a->flags & MGV_FLAG_GATED_SILU ? kActGated : kActNone;
   pl.bf16 = a->out_dtype == MGV_DTYPE_BF16;
 
-  const int want = (a->hints >> 8) & 31;
-  pl.pair = a->hints & MGV_GEMM_HINT_PAIR || (!(a->hints & MGV_GEMM_HINT_BLOCK) && a->M > 256);
-  if (pl.pair) plan_pair(pl, a->M, want ? std::min(256, (want + 1) / 2 * 32) : 0, sms, most);
-  else if ((st = plan_block(pl, a->M, want == 1 ? 16 : std::min(256, (want + 1) / 2 * 32), want ? (a->hints & 7) + 1 : 0, sms, most)) != MGV_STATUS_OK) return st;
+  if ((st = plan(pl, a, sms, most)) != MGV_STATUS_OK) return st;
   if ((st = encode_rows(&p.w_map, a->weights, a->N, a->K, a->ldw, kGemmRows)) != MGV_STATUS_OK) return st;
   return encode_rows(&p.x_map, a->x, a->M, a->K, a->ldx, pl.pair ? p.bt / 2 : p.bt);
 }

@@ -33,7 +33,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_pair_kernel(const __g
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.stages; ++i) bar_init(smem_u32(&sh.full[i]), 1), bar_init(smem_u32(&sh.empty[i]), 1);
-    for (int i = 0; i < 2; ++i) bar_init(smem_u32(&sh.ready[i]), 1), bar_init(smem_u32(&sh.drained[i]), 8);
+    for (int i = 0; i < 2; ++i) bar_init(smem_u32(&sh.ready[i]), 1), bar_init(smem_u32(&sh.drained[i]), 2 * kGemmEpilogue / 32);
     asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async;" ::: "memory");
   }
   if (warp == 1) {
@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_pair_kernel(const __g
       __syncwarp();
     }
   } else if (warp >= 2) {
-    const int quarter = warp % 4, row = int(rank) * kGemmRows + quarter * 32 + lane;
+    const int quarter = warp % 4, half = warp >= 6, row = int(rank) * kGemmRows + quarter * 32 + lane;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     uint32_t turn = 0;
     bool good = true;
@@ -126,18 +126,18 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_pair_kernel(const __g
       const uint32_t buf = turn & 1, lanes = tmem + buf * (p.tmem_cols / 2) + (uint32_t(quarter * 32) << 16);
       const Feature f = load_feature<BF16>(p, at.n0 + row);
       // the buffer's last readers have passed the barrier of the tile between
-      for (int i = threadIdx.x - 64; i < p.bt; i += 128) sh.x_scale[buf][i] = at.m0 + i < p.M ? p.x_scale[at.m0 + i] : 0.0f;
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (const int i = threadIdx.x - 64; i < p.bt) sh.x_scale[buf][i] = at.m0 + i < p.M ? p.x_scale[at.m0 + i] : 0.0f;
+      asm volatile("bar.sync 1, %0;" ::"n"(kGemmEpilogue) : "memory");
       good = good && bar_wait(smem_u32(&sh.ready[buf]), (turn >> 1) & 1, p.err);
       if (!good) continue;  // on to the barrier that the other warps wait at
       tmem_fence_after();
       const int columns = min(p.bt, p.M - at.m0);
-      for (int c = 0; c < columns; c += 16) {
+      for (int c = half * 16; c < columns; c += 32) {
         int v[16];
         __syncwarp();
         tmem_load16(lanes + c, v);
         tmem_wait_load();
-        finish16<ACT, BF16>(p, f, at.m0 + c, columns - c, v, sh.x_scale[buf] + c);
+        finish<ACT, BF16>(p, f, at.m0 + c, columns - c, v, sh.x_scale[buf] + c);
       }
       tmem_fence_before();
       __syncwarp();

@@ -25,6 +25,7 @@ struct GemmI8Params {
   int stages;      // ring slots
   int split;       // blocks of a cluster that share a tile's K range
   int n_tiles, m_tiles;
+  int sums_off;    // split: where the sums arrive in dynamic shared memory; 0: in the ring, once it is free
   uint32_t idesc;  // instruction descriptor of the matrix instruction
   uint32_t tmem_cols;
 };
@@ -32,7 +33,8 @@ struct GemmI8Params {
 constexpr int kGemmRows = 128;             // weight rows (output features) a block owns of a tile
 constexpr int kGemmK = 128;                // K of a ring slot: one 128-byte swizzle row
 constexpr int kGemmABytes = kGemmRows * kGemmK;
-constexpr int kGemmThreads = 192;          // producer warp, matrix warp, four epilogue warps
+constexpr int kGemmEpilogue = 256;         // threads of the epilogue: two warps for each 32 lanes of tensor memory
+constexpr int kGemmThreads = 64 + kGemmEpilogue;  // ... behind the producer warp and the matrix warp
 constexpr int kGemmMaxStages = 16;
 constexpr int kGemmAlign = 1024;           // of the ring; dynamic shared memory lost to it at most
 constexpr int kGemmReserved = 1024;        // shared memory the system takes for each block
@@ -42,7 +44,7 @@ constexpr int kGemmTimeout = 0x100;        // bit of the device error word
 // Static shared memory of the two kernels.
 struct GemmBlockShared {
   alignas(16) float x_scale[256];
-  uint64_t full[kGemmMaxStages], empty[kGemmMaxStages], done;
+  uint64_t full[kGemmMaxStages], empty[kGemmMaxStages], done, sums;
   uint32_t tmem_base;
   int failed;
 };
@@ -151,6 +153,16 @@ __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::l
 __device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
+template <bool RELEASE>  // whether what the block wrote before has to be seen behind the wait
+__device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();
+  if (RELEASE) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  else asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_sync() {
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -175,9 +187,12 @@ __device__ __forceinline__ void commit_pair(uint32_t bar) {
                "h"(uint16_t(3))
                : "memory");
 }
-// 16 bytes into the shared memory of a block of the cluster, and out of the own one
-__device__ __forceinline__ void store_cluster(uint32_t addr, int a, int b, int c, int d) {
-  asm volatile("st.shared::cluster.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+// 16 bytes into the shared memory of a block of the cluster, counted on that block's barrier `bar`
+// (both addresses in the cluster's window)
+__device__ __forceinline__ void send16(uint32_t addr, uint32_t bar, int a, int b, int c, int d) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%2,%3,%4,%5}, [%1];" ::"r"(addr), "r"(bar), "r"(a),
+               "r"(b), "r"(c), "r"(d)
+               : "memory");
 }
 __device__ __forceinline__ int4 load_shared(uint32_t addr) {
   int4 v;
@@ -215,15 +230,15 @@ __device__ __forceinline__ Feature load_feature(const GemmI8Params &p, int n) {
   return f;
 }
 
-// Sums of 16 neighbouring activation rows from m on for the lane's feature -- `rows` of them exist --
+// Sums of C neighbouring activation rows from m on for the lane's feature -- `rows` of them exist --
 // scaled, activated and stored.  Lanes 2i and 2i + 1 swap half of their values, so that the even
 // lane holds both features of the even rows and the odd lane both of the odd rows: one 32-bit store for two
 // features, or gate and up together.  All 32 lanes call it; x_scale is 16-byte aligned.
-template <int ACT, bool BF16>
-__device__ __forceinline__ void finish16(const GemmI8Params &p, const Feature &f, int m, int rows, const int (&v)[16], const float *x_scale) {
-  float y[16];
+template <int ACT, bool BF16, int C>
+__device__ __forceinline__ void finish(const GemmI8Params &p, const Feature &f, int m, int rows, const int (&v)[C], const float *x_scale) {
+  float y[C];
 #pragma unroll
-  for (int i = 0; i < 16; i += 4) {
+  for (int i = 0; i < C; i += 4) {
     const float4 s = *reinterpret_cast<const float4 *>(x_scale + i);
     y[i] = fmaf(float(v[i]), f.scale * s.x, f.bias);
     y[i + 1] = fmaf(float(v[i + 1]), f.scale * s.y, f.bias);
@@ -232,18 +247,18 @@ __device__ __forceinline__ void finish16(const GemmI8Params &p, const Feature &f
   }
   if (ACT == kActRelu || ACT == kActSilu) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) y[i] = ACT == kActSilu ? silu(y[i]) : y[i] < 0.0f ? 0.0f : y[i];
+    for (int i = 0; i < C; ++i) y[i] = ACT == kActSilu ? silu(y[i]) : y[i] < 0.0f ? 0.0f : y[i];
   }
   const int odd = f.n & 1;
   uint16_t *out = static_cast<uint16_t *>(p.out);
   if (ACT == kActGated || p.wide) {
-    float got[8];
+    float got[C / 2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) got[i] = __shfl_xor_sync(~0u, odd ? y[2 * i] : y[2 * i + 1], 1);
+    for (int i = 0; i < C / 2; ++i) got[i] = __shfl_xor_sync(~0u, odd ? y[2 * i] : y[2 * i + 1], 1);
     if (ACT == kActGated) {
       uint16_t *at = out + int64_t(m + odd) * p.ldd + (f.n >> 1);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < C / 2; ++i) {
         const float gate = odd ? got[i] : y[2 * i], up = odd ? y[2 * i + 1] : got[i];
         if (f.inside && 2 * i + odd < rows) *at = round_out<BF16>(silu(gate) * up);
         at += 2 * p.ldd;
@@ -252,7 +267,7 @@ __device__ __forceinline__ void finish16(const GemmI8Params &p, const Feature &f
       const bool both = (f.n | 1) < p.N, one = !both && (f.n & ~1) < p.N;  // the last feature of an odd N stands alone
       uint16_t *at = out + int64_t(m + odd) * p.ldd + (f.n & ~1);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < C / 2; ++i) {
         const uint32_t lo = round_out<BF16>(odd ? got[i] : y[2 * i]), hi = round_out<BF16>(odd ? y[2 * i + 1] : got[i]);
         if (both && 2 * i + odd < rows) *reinterpret_cast<uint32_t *>(at) = lo | hi << 16;
         if (one && 2 * i + odd < rows) *at = uint16_t(lo);
@@ -263,7 +278,7 @@ __device__ __forceinline__ void finish16(const GemmI8Params &p, const Feature &f
   }
   uint16_t *at = out + int64_t(m) * p.ldd + f.n;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < C; ++i) {
     if (f.inside && i < rows) *at = round_out<BF16>(y[i]);
     at += p.ldd;
   }
@@ -276,7 +291,8 @@ __device__ __forceinline__ void finish16(const GemmI8Params &p, const Feature &f
 struct GemmI8Plan {
   GemmI8Params p;
   int device = 0, grid = 0, smem = 0, cluster = 1, act = 0, bf16 = 0, flags = 0;
-  int pair = 0;  // the kernel of block pairs takes the call
+  int pair = 0;     // the kernel of block pairs takes the call
+  double cost = 0;  // estimated cycles
 };
 
 // Launches KERN as the plan says; its first launch on a device lifts its shared-memory limit.
