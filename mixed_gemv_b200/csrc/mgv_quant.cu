@@ -185,6 +185,8 @@ __device__ __forceinline__ RowStats block_stats(RowStats s, RowStats *buf) {
   return warp_stats(r);
 }
 
+constexpr int kLongThreads = 512;
+
 // Marks, in its place in `scale`, a row that is left for row_in_double.
 constexpr float kLeft = -1.0f;
 
@@ -195,7 +197,7 @@ constexpr float kLeft = -1.0f;
 // values to a thread, then the next one; the norm's weights stay in registers over its rows.
 template <typename T, bool NORM, int V, int NV, bool WARP_ROW>
 __global__ void __launch_bounds__(WARP_ROW ? 128 : 1024, WARP_ROW ? 6 : 1) rows_kernel(const __grid_constant__ RowParams p) {
-  constexpr bool kKeepWeight = NV <= 2;
+  constexpr bool kKeepWeight = NV <= 2 || (V == 1 && NV == 8);
   constexpr int kWords = V == 8 ? 4 : 1;
   using P = Piece<V>;
   __shared__ RowStats stats[2][32];
@@ -213,41 +215,50 @@ __global__ void __launch_bounds__(WARP_ROW ? 128 : 1024, WARP_ROW ? 6 : 1) rows_
     }
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  const bool add = NORM && p.residual;
+  // Where registers allow it the next row is on its way while this one is reduced.
+  constexpr bool kAhead = V == 8 && !WARP_ROW && NV <= (NORM ? 2 : 4);
+  constexpr int kGroup = NV < 4 ? NV : 4;  // pieces of the residual in flight
+  P h[NV], r[kGroup];
+  auto load = [&](P *to, int count, int from, const void *rows, int64_t ld, int64_t m) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (i >= count) break;
+      const int k = ((from + i) * step + t) * V;
+      if (k < p.K) to[i] = load_piece<V>(static_cast<const T *>(rows) + m * ld, k, p.K - k);
+    }
+  };
+  if (kAhead && first < p.M) {
+    load(h, NV, 0, p.x, p.ldx, first);
+    if (add) load(r, kGroup, 0, p.residual, p.ldr, first);
+  }
   int turn = 0;
   bool left = false;
   for (int64_t m = first; m < p.M; m += stride, turn ^= 1) {
-    const T *x = static_cast<const T *>(p.x) + m * p.ldx;
-    P h[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int k = (i * step + t) * V;
-      if (k < p.K) h[i] = load_piece<V>(x, k, p.K - k);
-    }
-    if (NORM && p.residual) {
-      const T *r = static_cast<const T *>(p.residual) + m * p.ldr;
+    if (!kAhead) load(h, NV, 0, p.x, p.ldx, m);
+    if (add) {
       T *ro = static_cast<T *>(p.residual_out) + m * p.ldro;
-      constexpr int kGroup = NV < 4 ? NV : 4;  // loads in flight, within the registers there are
-      P add[kGroup];
 #pragma unroll
       for (int g = 0; g < NV; g += kGroup) {
-#pragma unroll
-        for (int i = 0; i < kGroup; ++i) {
-          const int k = ((g + i) * step + t) * V;
-          if (k < p.K) add[i] = load_piece<V>(r, k, p.K - k);
-        }
+        if (!kAhead) load(r, kGroup, g, p.residual, p.ldr, m);
 #pragma unroll
         for (int i = 0; i < kGroup; ++i) {
           const int k = ((g + i) * step + t) * V;
           if (k < p.K) {
 #pragma unroll
             for (int j = 0; j < kWords; ++j) {
-              const float2 a = unpack2<T>(h[g + i].u[j]), b = unpack2<T>(add[i].u[j]);
-              h[g + i].u[j] = pack2<T>(a.x + b.x, a.y + b.y);
+              const float2 u = unpack2<T>(h[g + i].u[j]), v = unpack2<T>(r[i].u[j]);
+              h[g + i].u[j] = pack2<T>(u.x + v.x, u.y + v.y);
             }
             store_piece<V>(ro, k, h[g + i], p.K - k);
           }
         }
       }
+    }
+    P next[kAhead ? NV : 1];
+    if (kAhead && m + stride < p.M) {
+      load(next, NV, 0, p.x, p.ldx, m + stride);
+      if (add) load(r, kGroup, 0, p.residual, p.ldr, m + stride);
     }
     RowStats s = {0.0f, 0u};
 #pragma unroll
@@ -272,19 +283,19 @@ __global__ void __launch_bounds__(WARP_ROW ? 128 : 1024, WARP_ROW ? 6 : 1) rows_
     }
     s = WARP_ROW ? warp_stats(s) : block_stats(s, stats[turn]);
     const float mean = s.ss / float(p.K) + p.eps;
-    if (!row_is_tame<NORM>(p, s, mean)) {
+    const bool tame = row_is_tame<NORM>(p, s, mean);
+    if (!tame) {
       if (t == 0) p.scale[m] = kLeft;
       left = true;
-      continue;
     }
     float scale, inv;
     row_factors<NORM>(s, mean, scale, inv);
-    if (t == 0) p.scale[m] = scale;
+    if (t == 0 && tame) p.scale[m] = scale;
     int8_t *q = p.q + m * p.ldq;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int k = (i * step + t) * V;
-      if (k < p.K) {
+      if (k < p.K && tame) {
         P wi = {};
         if (NORM) wi = kKeepWeight ? w[kKeepWeight ? i : 0] : load_piece<V>(p.weight, k, p.K - k);
         float2 y[kWords];
@@ -308,6 +319,10 @@ __global__ void __launch_bounds__(WARP_ROW ? 128 : 1024, WARP_ROW ? 6 : 1) rows_
         }
       }
     }
+    if (kAhead) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) h[i] = next[i];
+    }
   }
   if (!left) return;  // the same for all threads of a row
   if (WARP_ROW) __syncwarp();
@@ -318,41 +333,69 @@ __global__ void __launch_bounds__(WARP_ROW ? 128 : 1024, WARP_ROW ? 6 : 1) rows_
 
 // Rows too long for registers: a block per row, value by value, in two passes over it.
 template <typename T, bool NORM>
-__global__ void __launch_bounds__(1024, 1) long_rows_kernel(const __grid_constant__ RowParams p) {
+__global__ void __launch_bounds__(kLongThreads, 3) long_rows_kernel(const __grid_constant__ RowParams p) {
   __shared__ RowStats stats[32];
   __shared__ double buf[32];
   const int64_t m = blockIdx.x;
   const T *x = static_cast<const T *>(p.x) + m * p.ldx, *w = static_cast<const T *>(p.weight);
+  const bool add = NORM && p.residual;
+  const T *r = add ? static_cast<const T *>(p.residual) + m * p.ldr : nullptr;
+  T *ro = add ? static_cast<T *>(p.residual_out) + m * p.ldro : nullptr;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const T *h = x;
   RowStats s = {0.0f, 0u};
-  if (NORM && p.residual) {
-    const T *r = static_cast<const T *>(p.residual) + m * p.ldr;
-    T *ro = static_cast<T *>(p.residual_out) + m * p.ldro;
-    for (int k = threadIdx.x; k < p.K; k += blockDim.x) ro[k] = from_f<T>(to_f(x[k]) + to_f(r[k]));
-    h = ro;  // every thread reads back what it wrote
-  }
-#pragma unroll 4
-  for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
-    const float v = to_f(h[k]), y = NORM ? v * to_f(w[k]) : v;
-    if (NORM) s.ss = fmaf(v, v, s.ss);
-    s.top = max(s.top, __float_as_uint(y) & 0x7fffffffu);
+  constexpr int kBatch = 8;  // loads in flight
+  for (int k0 = threadIdx.x; k0 < p.K; k0 += kBatch * kLongThreads) {
+    T h[kBatch], a[kBatch], g[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int k = k0 + j * kLongThreads;
+      if (k < p.K) {
+        h[j] = x[k];
+        if (NORM) g[j] = w[k];
+        if (add) a[j] = r[k];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int k = k0 + j * kLongThreads;
+      if (k < p.K) {
+        if (add) ro[k] = h[j] = from_f<T>(to_f(h[j]) + to_f(a[j]));
+        const float v = to_f(h[j]), y = NORM ? v * to_f(g[j]) : v;
+        if (NORM) s.ss = fmaf(v, v, s.ss);
+        s.top = max(s.top, __float_as_uint(y) & 0x7fffffffu);
+      }
+    }
   }
   s = block_stats(s, stats);
   const float mean = s.ss / float(p.K) + p.eps;
   if (!row_is_tame<NORM>(p, s, mean)) {
-    row_in_double<T, NORM, false>(p, m, threadIdx.x, blockDim.x, buf);
+    row_in_double<T, NORM, false>(p, m, threadIdx.x, kLongThreads, buf);
     return;
   }
   float scale, inv;
   row_factors<NORM>(s, mean, scale, inv);
   if (threadIdx.x == 0) p.scale[m] = scale;
+  const T *again = add ? ro : x;  // every thread reads back what it wrote
   int8_t *q = p.q + m * p.ldq;
-#pragma unroll 4
-  for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
-    const float v = to_f(h[k]);
-    q[k] = int8_t(__float_as_uint(fmaf(NORM ? v * to_f(w[k]) : v, inv, kRoundMagic)) & 0xff);
+  for (int k0 = threadIdx.x; k0 < p.K; k0 += kBatch * kLongThreads) {
+    T h[kBatch], g[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int k = k0 + j * kLongThreads;
+      if (k < p.K) {
+        h[j] = again[k];
+        if (NORM) g[j] = w[k];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int k = k0 + j * kLongThreads;
+      if (k < p.K) {
+        const float v = to_f(h[j]);
+        q[k] = int8_t(__float_as_uint(fmaf(NORM ? v * to_f(g[j]) : v, inv, kRoundMagic)) & 0xff);
+      }
+    }
   }
 }
 
@@ -366,10 +409,12 @@ struct BackParams {
 
 constexpr int kBackThreads = 256;
 
-// One piece of V values per thread and row group; a block takes kBackThreads / lanes rows at a time.
+// 16 neighbouring values to a thread (V = 16), or eight that are p.lanes apart (V = 1); a block takes
+// kBackThreads / lanes rows.
 template <typename T, int V>
 __global__ void __launch_bounds__(kBackThreads) back_kernel(const BackParams p) {
-  const int rows = kBackThreads / p.lanes, row = threadIdx.x / p.lanes, width = p.lanes * V;
+  constexpr int kEach = V == 1 ? 8 : V;
+  const int rows = kBackThreads / p.lanes, row = threadIdx.x / p.lanes, width = p.lanes * kEach;
   const int64_t chunks = (p.K + width - 1) / width;
   const int64_t m = int64_t(blockIdx.x / chunks) * rows + row;
   const int k = int(blockIdx.x % chunks) * width + (threadIdx.x % p.lanes) * V;
@@ -380,7 +425,15 @@ __global__ void __launch_bounds__(kBackThreads) back_kernel(const BackParams p) 
   const float s = p.scale[m];
   T *out = static_cast<T *>(p.out) + m * p.ldo + k;
   const int8_t *q = p.q + m * p.ldq + k;
-  if (V == 16 && n >= V) {
+  if (V == 1) {
+    float f[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (j * p.lanes < n) f[j] = float(q[j * p.lanes]);
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (j * p.lanes < n) out[j * p.lanes] = from_f<T>(f[j] * s);
+  } else if (n >= V) {
     const uint4 b = *reinterpret_cast<const uint4 *>(q);
     const uint32_t word[4] = {b.x, b.y, b.z, b.w};
     uint32_t o[8];
@@ -396,7 +449,7 @@ __global__ void __launch_bounds__(kBackThreads) back_kernel(const BackParams p) 
     reinterpret_cast<uint4 *>(out)[0] = make_uint4(o[0], o[1], o[2], o[3]);
     reinterpret_cast<uint4 *>(out)[1] = make_uint4(o[4], o[5], o[6], o[7]);
   } else {
-    for (int j = 0; j < V && j < n; ++j) out[j] = from_f<T>(float(q[j]) * s);
+    for (int j = 0; j < n; ++j) out[j] = from_f<T>(float(q[j]) * s);
   }
 }
 
@@ -434,16 +487,17 @@ static mgv_status quantise(const RowParams &p, int flags, cudaStream_t s) {
                     (!NORM || (aligned_rows(p.weight, 0, 2, 1, 16) &&
                                (!p.residual || (aligned_rows(p.residual, p.ldr, 2, p.M, 16) && aligned_rows(p.residual_out, p.ldro, 2, p.M, 16)))));
   const int sms = sm_count();
+  const int64_t few = 2 * int64_t(sms);
   if (wide && p.K <= 65536) {
     const int pieces = (p.K + 7) / 8;
-    const int64_t few = 2 * int64_t(sms);
     if (pieces <= 128 && p.M > few)
       return launch_rows(rows_kernel<T, NORM, 8, 4, true>, std::min<int64_t>((p.M + 3) / 4, int64_t(sms) * 16), 128, flags, s, p);
-    // few rows: as many threads as a row has pieces, for the shortest chain of loads; many rows: four pieces a
-    // thread, so that several blocks of an SM are at different points of their rows
+    // few rows: as many threads as a row has pieces, for the shortest chain of loads; many rows: more pieces a thread and
+    // smaller blocks, so that several of an SM are at different points of their rows (norm of 4096 x 8192 with residual
+    // 42.9 us with four pieces, 37.8 with two and the next row on its way; quantisation 22.9 us with two, 16.5 with four)
     int nv = 1;
     while (nv < 8 && pieces > 1024 * nv) nv *= 2;
-    if (p.M > few) nv = std::max(nv, 4);
+    if (p.M > few) nv = std::max(nv, NORM ? 2 : 4);
     const int threads = std::max(32, ((pieces + nv - 1) / nv + 31) / 32 * 32);
     const int64_t grid = std::min<int64_t>(p.M, int64_t(sms) * std::max(1, 2048 / threads));
     switch (nv) {
@@ -453,18 +507,19 @@ static mgv_status quantise(const RowParams &p, int flags, cudaStream_t s) {
       default: return launch_rows(rows_kernel<T, NORM, 8, 8, false>, grid, threads, flags, s, p);
     }
   }
-  if (p.K <= 8192) {
-    const int threads = std::max(32, ((p.K + 7) / 8 + 31) / 32 * 32);
-    const int64_t grid = std::min<int64_t>(p.M, int64_t(sms) * std::max(1, 2048 / threads));
-    return launch_rows(rows_kernel<T, NORM, 1, 8, false>, grid, threads, flags, s, p);
+  // Value by value: in registers where rows are short or few, else in two passes (the norm of 1000 rows of 5001:
+  // 16.6 us against 22.5).
+  if (p.K <= 2048 || (p.K <= 8192 && p.M <= few)) {
+    const int threads = ((p.K + 7) / 8 + 31) / 32 * 32;
+    return launch_rows(rows_kernel<T, NORM, 1, 8, false>, std::min<int64_t>(p.M, int64_t(sms) * (2048 / threads)), threads, flags, s, p);
   }
-  return launch_rows(long_rows_kernel<T, NORM>, p.M, 1024, flags, s, p);
+  return launch_rows(long_rows_kernel<T, NORM>, p.M, kLongThreads, flags, s, p);
 }
 
 template <typename T>
 static mgv_status dequantise(BackParams p, int flags, cudaStream_t s) {
   const bool wide = aligned_rows(p.q, p.ldq, 1, p.M, 16) && aligned_rows(p.out, p.ldo, 2, p.M, 16);
-  const int v = wide ? 16 : 1;
+  const int v = wide ? 16 : 8;
   p.lanes = 1;
   while (p.lanes < kBackThreads && p.lanes * v < p.K) p.lanes *= 2;
   const int rows = kBackThreads / p.lanes;
