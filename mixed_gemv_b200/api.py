@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass
+from functools import partial
 from typing import Optional, Sequence
 
 import torch
@@ -389,10 +390,10 @@ class _RowOperator:
     def run(self, stream=None) -> None:
         if self._call is None:
             raise MgvError(1, f"{type(self).__name__}.run() before initialize()")
-        if torch.cuda.current_device() != self._device:
-            raise MgvError(1, f"{type(self).__name__} was initialized for device {self._device}, "
-                              f"current is {torch.cuda.current_device()}")
-        status = self._call(_stream_ptr(stream))
+        current = torch.cuda.current_device()
+        if current != self._device:
+            raise MgvError(1, f"{type(self).__name__} was initialized for device {self._device}, current is {current}")
+        status = self._call(_current_raw_stream(current) if stream is None and _current_raw_stream else _stream_ptr(stream))
         if status:
             check(status)
 
@@ -417,7 +418,7 @@ class RowQuantizer(_RowOperator):
         q = _rows(a.q, "q", (M, K), (torch.int8,), a.x.device)
         scale = _rows(a.scale, "scale", (M,), (torch.float32,), a.x.device)
         fixed = _as_c(lib.mgv_quantize_rows, q, scale, x, int(_DTYPES[a.x.dtype]), M, K, _ld(a.q), _ld(a.x), int(a.flags))
-        return a.x.device.index, lambda s: lib.mgv_quantize_rows(*fixed, s)
+        return a.x.device.index, partial(lib.mgv_quantize_rows, *fixed)
 
 
 @dataclass
@@ -436,7 +437,7 @@ class RowDequantizer(_RowOperator):
         scale = _rows(a.scale, "scale", (M,), (torch.float32,), a.q.device)
         out = _rows(a.out, "out", (M, K), (torch.float16, torch.bfloat16), a.q.device)
         fixed = _as_c(lib.mgv_dequantize_rows, out, q, scale, int(_DTYPES[a.out.dtype]), M, K, _ld(a.out), _ld(a.q), int(a.flags))
-        return a.q.device.index, lambda s: lib.mgv_dequantize_rows(*fixed, s)
+        return a.q.device.index, partial(lib.mgv_dequantize_rows, *fixed)
 
 
 @dataclass
@@ -471,8 +472,7 @@ class RmsNormQuantizer(_RowOperator):
             c.ldr, c.ldro = _ld(a.residual), _ld(a.residual_out)
         c.dtype, c.flags, c.M, c.K = int(_DTYPES[a.x.dtype]), int(a.flags), M, K
         c.ldx, c.ldq, c.eps = _ld(a.x), _ld(a.q), float(a.eps)
-        ref = C.byref(c)
-        return dev.index, lambda s: lib.mgv_rmsnorm_quantize(ref, s)
+        return dev.index, partial(lib.mgv_rmsnorm_quantize, C.pointer(c))
 
 
 @dataclass
@@ -536,4 +536,4 @@ class GemmI8Adaptor(_RowOperator):
         plan = C.c_void_p()
         check(lib.mgv_gemm_i8_plan_create(C.byref(c), C.byref(plan)))
         self._plan = plan
-        return a.x.device.index, lambda s: lib.mgv_gemm_i8_plan_run(plan, s)
+        return a.x.device.index, partial(lib.mgv_gemm_i8_plan_run, plan)

@@ -17,7 +17,7 @@ namespace mgv {
 constexpr int kQuadBytes = kGemmRows * 16;  // sums of 128 features x 4 columns
 
 template <int ACT, bool BF16>
-__global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_block_kernel(const __grid_constant__ GemmI8Params p) {
+__global__ void __launch_bounds__(kGemmThreads, kGemmBlocksPerSm) gemm_i8_block_kernel(const __grid_constant__ GemmI8Params p) {
   extern __shared__ uint8_t dynamic[];
   __shared__ GemmBlockShared sh;
   const uint32_t ring = (smem_u32(dynamic) + 1023) & ~1023u;
@@ -116,15 +116,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_block_kernel(const __
     asm volatile("bar.sync 1, %0;" ::"n"(kGemmEpilogue) : "memory");
     good = bar_wait(smem_u32(&sh.done), 0, p.err) && !*static_cast<volatile int *>(&sh.failed);
     tmem_fence_after();
-    if (p.split == 1 && good) {
-      for (int c = half * 16; c < columns; c += 32) {
-        int v[16];
-        __syncwarp();
-        tmem_load16(lanes + c, v);
-        tmem_wait_load();
-        finish<ACT, BF16>(p, f, m0 + c, columns - c, v, sh.x_scale + c);
-      }
-    }
+    if (p.split == 1 && good) finish_columns<ACT, BF16>(p, f, lanes, m0, half * 16, columns, sh.x_scale);
   }
   if (p.split > 1) {
     // Block r finishes the column quads r, r + split, ...; of each it gets [128 features][4 columns] from
@@ -138,7 +130,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_block_kernel(const __
         int v[16];
         __syncwarp();
         tmem_load16(lanes + c, v);
-        tmem_wait_load();
+        tmem_wait(v);
         int owner = c / 4 % p.split, at = c / 4 - owner + int(rank);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -285,7 +277,7 @@ static void plan_block(GemmI8Plan &pl, int64_t M, int bt, int split, int sms, in
   // its allocation for another to end: at least the same fraction of both.
   const int fixed = kGemmReserved + int(sizeof(GemmBlockShared));  // beside the dynamic part; kGemmAlign of that goes to alignment
   const int64_t on_sm = (grid + sms - 1) / sms;
-  int per_sm = int(std::max<int64_t>(bt <= 64 ? 2 : 1, std::min<int64_t>(on_sm, 512 / p.tmem_cols)));
+  int per_sm = int(std::max<int64_t>(bt <= 64 ? 2 : 1, std::min<int64_t>(std::min<int64_t>(on_sm, kGemmBlocksPerSm), 512 / p.tmem_cols)));
   while (per_sm > 1 && (kGemmSmShared / per_sm - fixed - kGemmAlign) / slot < std::min(3, share)) --per_sm;
   const int room = std::min(kGemmSmShared / per_sm - fixed, most - int(sizeof(GemmBlockShared))) - kGemmAlign;
   p.stages = std::min(std::min(share, kGemmMaxStages), room / slot);
@@ -304,7 +296,7 @@ static void plan_block(GemmI8Plan &pl, int64_t M, int bt, int split, int sms, in
   pl.smem = smem;
   pl.grid = int(std::min<int64_t>(grid, 0x7fffffff));
   pl.cluster = split;
-  const int64_t at_once = std::max(1, std::min(kGemmSmShared / (smem + fixed), int(512 / p.tmem_cols)));
+  const int64_t at_once = std::max(1, std::min(std::min(kGemmSmShared / (smem + fixed), int(512 / p.tmem_cols)), kGemmBlocksPerSm));
   const double slice = std::max(slot / kSmBytes, 4 * std::max(40.0, bt / 2.0));  // of the SM's time
   const double tail = split > 1 ? 1500 + 45.0 * bt : kColumn16 * ((bt + 15) / 16);
   const int64_t rounds = (on_sm + at_once - 1) / at_once;  // blocks that follow one another: each starts and ends alone

@@ -132,13 +132,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_pair_kernel(const __g
       if (!good) continue;  // on to the barrier that the other warps wait at
       tmem_fence_after();
       const int columns = min(p.bt, p.M - at.m0);
-      for (int c = half * 16; c < columns; c += 32) {
-        int v[16];
-        __syncwarp();
-        tmem_load16(lanes + c, v);
-        tmem_wait_load();
-        finish<ACT, BF16>(p, f, at.m0 + c, columns - c, v, sh.x_scale[buf] + c);
-      }
+      finish_columns<ACT, BF16>(p, f, lanes, at.m0, half * 16, columns, sh.x_scale[buf]);
       tmem_fence_before();
       __syncwarp();
       if (lane == 0) arrive_in_block(in_block(smem_u32(&sh.drained[buf]), 0));

@@ -35,6 +35,7 @@ constexpr int kGemmK = 128;                // K of a ring slot: one 128-byte swi
 constexpr int kGemmABytes = kGemmRows * kGemmK;
 constexpr int kGemmEpilogue = 256;         // threads of the epilogue: two warps for each 32 lanes of tensor memory
 constexpr int kGemmThreads = 64 + kGemmEpilogue;  // ... behind the producer warp and the matrix warp
+constexpr int kGemmBlocksPerSm = 3;        // of the single-block kernel, by its registers
 constexpr int kGemmMaxStages = 16;
 constexpr int kGemmAlign = 1024;           // of the ring; dynamic shared memory lost to it at most
 constexpr int kGemmReserved = 1024;        // shared memory the system takes for each block
@@ -141,7 +142,7 @@ __device__ __forceinline__ void multiply_add(uint32_t d, uint64_t a, uint64_t b,
         : "memory");
 }
 
-// 16 accumulator columns of the warp's 32 lanes.
+// 16 accumulator columns of the warp's 32 lanes; the registers hold them behind tmem_wait only.
 __device__ __forceinline__ void tmem_load16(uint32_t addr, int (&v)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -149,7 +150,11 @@ __device__ __forceinline__ void tmem_load16(uint32_t addr, int (&v)[16]) {
         "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
       : "r"(addr));
 }
-__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait(int (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]),
+                 "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])::"memory");
+}
 __device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
@@ -281,6 +286,19 @@ __device__ __forceinline__ void finish(const GemmI8Params &p, const Feature &f, 
   for (int i = 0; i < C; ++i) {
     if (f.inside && i < rows) *at = round_out<BF16>(y[i]);
     at += p.ldd;
+  }
+}
+
+// The 16-column groups at c, c + 32, ... of a tile from row m0 on, out of the warp's lanes of tensor
+// memory.  (Fetching the next group while one is finished gained nothing and took 30 registers more.)
+template <int ACT, bool BF16>
+__device__ __forceinline__ void finish_columns(const GemmI8Params &p, const Feature &f, uint32_t lanes, int m0, int c, int columns, const float *x_scale) {
+  for (; c < columns; c += 32) {
+    int v[16];
+    __syncwarp();
+    tmem_load16(lanes + c, v);
+    tmem_wait(v);
+    finish<ACT, BF16>(p, f, m0 + c, columns - c, v, x_scale + c);
   }
 }
 
