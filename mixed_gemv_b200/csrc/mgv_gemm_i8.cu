@@ -317,12 +317,21 @@ static void plan_pair(GemmI8Plan &pl, int64_t M, int bt, int sms, int most) {
   const int64_t tiles = int64_t(p.n_tiles) * p.m_tiles, pairs = std::min<int64_t>(tiles, sms / 2);
   const int slices = (p.K + kGemmK - 1) / kGemmK, slot = kGemmABytes + bt / 2 * kGemmK, room = most - int(sizeof(GemmPairShared));
   p.stages = std::min(kGemmMaxStages, (room - kGemmAlign) / slot);
+  // the last round's tiles in halves where those are enough for no more than a round of their own
+  const int64_t rounds = tiles / pairs, rest = tiles % pairs;
+  const bool halve = rounds > 0 && rest > 0 && 2 * rest <= pairs && bt % 64 == 0;
+  p.halved = int(halve ? tiles - rest : tiles);
+  p.half_idesc = instruction(2 * kGemmRows, halve ? bt / 2 : bt);
   pl.pair = 1;
   pl.smem = room;  // one block per SM: it may hold all of the tensor memory
   pl.grid = int(2 * pairs);
   pl.cluster = 2;
-  const double slice = std::max(std::max(slot / kSmBytes, kIssue), 2.0 * bt), tail = kColumn16 * (bt / 16);
-  const double chain = double((tiles + pairs - 1) / pairs) * std::max(slices * slice, tail);  // a tile's epilogue beside the next tile
+  auto round = [&](int rows) {  // a tile's epilogue runs beside the next tile
+    const double slice = std::max(std::max((kGemmABytes + rows / 2 * kGemmK) / kSmBytes, kIssue), 2.0 * rows);
+    return std::max(slices * slice, kColumn16 * (rows / 16));
+  };
+  const double tail = kColumn16 * ((halve ? bt / 2 : bt) / 16);
+  const double chain = rounds * round(bt) + (halve ? round(bt / 2) : rest ? round(bt) : 0);
   pl.cost = estimate(chain, 2.0 * tiles * slices * slot / kPairBytes, double(p.N) * p.K, tail);
 }
 
@@ -382,6 +391,7 @@ static mgv_status prepare(const mgv_gemm_i8_args *a, mgv_gemm_i8_plan &pl) {
 
   if ((st = plan(pl, a, sms, most)) != MGV_STATUS_OK) return st;
   if ((st = encode_rows(&p.w_map, a->weights, a->N, a->K, a->ldw, kGemmRows)) != MGV_STATUS_OK) return st;
+  if (pl.pair && p.halved < p.n_tiles * p.m_tiles && (st = encode_rows(&p.x_half_map, a->x, a->M, a->K, a->ldx, p.bt / 4)) != MGV_STATUS_OK) return st;
   return encode_rows(&p.x_map, a->x, a->M, a->K, a->ldx, pl.pair ? p.bt / 2 : p.bt);
 }
 

@@ -8,18 +8,23 @@ namespace mgv {
 constexpr int kGemmBand = 8;
 
 struct TileAt {
-  int n0, m0;
+  int n0, m0, rows;
 };
-__device__ __forceinline__ TileAt tile_at(const GemmI8Params &p, uint32_t tile) {
+// The item of that number in the order of work: a tile, or half the rows of one.
+__device__ __forceinline__ TileAt tile_at(const GemmI8Params &p, uint32_t item) {
+  const uint32_t whole = uint32_t(p.halved), tile = item < whole ? item : whole + (item - whole) / 2;
   const uint32_t per_band = uint32_t(kGemmBand) * p.n_tiles, band = tile / per_band, in = tile % per_band;
   const uint32_t height = min(uint32_t(kGemmBand), uint32_t(p.m_tiles) - band * kGemmBand);
-  return {int(in / height) * 2 * kGemmRows, int(band * kGemmBand + in % height) * p.bt};
+  const int n0 = int(in / height) * 2 * kGemmRows, m0 = int(band * kGemmBand + in % height) * p.bt;
+  if (item < whole) return {n0, m0, p.bt};
+  return {n0, m0 + int((item - whole) % 2) * (p.bt / 2), p.bt / 2};
 }
 
 // Persistent: a pair of blocks (two SMs) per tile of 256 output features x p.bt activation rows.  Each
 // block holds 128 of the features and copies half of the rows; one thread of the first block issues
 // matrix instructions for both.  Two accumulators in tensor memory: the epilogue of a tile runs
-// beside the next tile's products.
+// beside the next tile's products.  Where the last round of tiles would leave half of the pairs or more without
+// one, its tiles are halved: 2048 x 8192 features at 256 rows are 3.46 tiles to a pair, in 3.5 rounds instead of 4.
 template <int ACT, bool BF16>
 __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_pair_kernel(const __grid_constant__ GemmI8Params p) {
   extern __shared__ uint8_t dynamic[];
@@ -27,9 +32,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_pair_kernel(const __g
   const uint32_t ring = (smem_u32(dynamic) + 1023) & ~1023u;
   const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const uint32_t rank = cluster_rank();
-  const uint32_t pairs = gridDim.x / 2, pair = blockIdx.x / 2, tiles = uint32_t(p.n_tiles) * uint32_t(p.m_tiles);
+  const uint32_t pairs = gridDim.x / 2, pair = blockIdx.x / 2, items = 2 * uint32_t(p.n_tiles) * uint32_t(p.m_tiles) - uint32_t(p.halved);
   const int slices = (p.K + kGemmK - 1) / kGemmK;
-  const uint32_t slot_bytes = kGemmABytes + p.bt / 2 * kGemmK;
+  const uint32_t slot_bytes = kGemmABytes + p.bt / 2 * kGemmK;  // of whole tiles
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.stages; ++i) bar_init(smem_u32(&sh.full[i]), 1), bar_init(smem_u32(&sh.empty[i]), 1);
@@ -55,18 +60,18 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_pair_kernel(const __g
     const int ahead = min(slices, p.stages);
     if (one) {
       for (int i = 0; i < ahead; ++i) {
-        if (rank == 0) bar_expect(smem_u32(&sh.full[i]), 2 * slot_bytes);
+        if (rank == 0) bar_expect(smem_u32(&sh.full[i]), 2 * kGemmABytes + at.rows * kGemmK);
         box_load_pair(ring + i * slot_bytes, &p.w_map, i * kGemmK, at.n0 + int(rank) * kGemmRows, in_block(smem_u32(&sh.full[i]), 0));
       }
     }
     asm volatile("griddepcontrol.wait;\n\tfence.proxy.async.global;" ::: "memory");
     if (one)
       for (int i = 0; i < ahead; ++i)
-        box_load_pair(ring + i * slot_bytes + kGemmABytes, &p.x_map, i * kGemmK, at.m0 + int(rank) * p.bt / 2, in_block(smem_u32(&sh.full[i]), 0));
+        box_load_pair(ring + i * slot_bytes + kGemmABytes, at.rows == p.bt ? &p.x_map : &p.x_half_map, i * kGemmK, at.m0 + int(rank) * at.rows / 2, in_block(smem_u32(&sh.full[i]), 0));
     int slot = ahead % p.stages;
     uint32_t issued = ahead, phase = 0;  // phase: of `empty` once the ring is full
     bool ok = true;
-    for (uint32_t tile = pair; tile < tiles && ok; tile += pairs) {
+    for (uint32_t tile = pair; tile < items && ok; tile += pairs) {
       at = tile_at(p, tile);
       for (int i = tile == pair ? ahead : 0; i < slices; ++i) {
         if (issued >= uint32_t(p.stages)) {
@@ -76,9 +81,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_pair_kernel(const __g
         }
         if (one) {
           const uint32_t bar = in_block(smem_u32(&sh.full[slot]), 0), dst = ring + slot * slot_bytes;
-          if (rank == 0) bar_expect(smem_u32(&sh.full[slot]), 2 * slot_bytes);
+          if (rank == 0) bar_expect(smem_u32(&sh.full[slot]), 2 * kGemmABytes + at.rows * kGemmK);
           box_load_pair(dst, &p.w_map, i * kGemmK, at.n0 + int(rank) * kGemmRows, bar);
-          box_load_pair(dst + kGemmABytes, &p.x_map, i * kGemmK, at.m0 + int(rank) * p.bt / 2, bar);
+          box_load_pair(dst + kGemmABytes, at.rows == p.bt ? &p.x_map : &p.x_half_map, i * kGemmK, at.m0 + int(rank) * at.rows / 2, bar);
         }
         if (++slot == p.stages) slot = 0;
         ++issued;
@@ -96,8 +101,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_pair_kernel(const __g
     int slot = 0;
     uint32_t phase = 0, turn = 0;
     bool ok = true;
-    for (uint32_t tile = pair; tile < tiles && ok; tile += pairs, ++turn) {
-      const uint32_t buf = turn & 1, acc = tmem + buf * (p.tmem_cols / 2);
+    for (uint32_t tile = pair; tile < items && ok; tile += pairs, ++turn) {
+      const uint32_t buf = turn & 1, acc = tmem + buf * (p.tmem_cols / 2), idesc = tile < uint32_t(p.halved) ? p.idesc : p.half_idesc;
       if (turn >= 2) ok = bar_wait<true>(smem_u32(&sh.drained[buf]), ((turn >> 1) - 1) & 1, p.err);
       tmem_fence_after();
       for (int i = 0; i < slices && ok; ++i) {
@@ -107,7 +112,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_pair_kernel(const __g
         const uint64_t a = operand_desc(ring + slot * slot_bytes), b = operand_desc(ring + slot * slot_bytes + kGemmABytes);
         if (one) {
 #pragma unroll
-          for (int k = 0; k < kGemmK / 32; ++k) multiply_add<2>(acc, a + 2 * k, b + 2 * k, p.idesc, i + k > 0);
+          for (int k = 0; k < kGemmK / 32; ++k) multiply_add<2>(acc, a + 2 * k, b + 2 * k, idesc, i + k > 0);
           commit_pair(smem_u32(&sh.empty[slot]));
         }
         __syncwarp();
@@ -121,17 +126,17 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_pair_kernel(const __g
     asm volatile("griddepcontrol.wait;" ::: "memory");
     uint32_t turn = 0;
     bool good = true;
-    for (uint32_t tile = pair; tile < tiles; tile += pairs, ++turn) {
+    for (uint32_t tile = pair; tile < items; tile += pairs, ++turn) {
       const TileAt at = tile_at(p, tile);
       const uint32_t buf = turn & 1, lanes = tmem + buf * (p.tmem_cols / 2) + (uint32_t(quarter * 32) << 16);
       const Feature f = load_feature<BF16>(p, at.n0 + row);
       // the buffer's last readers have passed the barrier of the tile between
-      if (const int i = threadIdx.x - 64; i < p.bt) sh.x_scale[buf][i] = at.m0 + i < p.M ? p.x_scale[at.m0 + i] : 0.0f;
+      if (const int i = threadIdx.x - 64; i < at.rows) sh.x_scale[buf][i] = at.m0 + i < p.M ? p.x_scale[at.m0 + i] : 0.0f;
       asm volatile("bar.sync 1, %0;" ::"n"(kGemmEpilogue) : "memory");
       good = good && bar_wait(smem_u32(&sh.ready[buf]), (turn >> 1) & 1, p.err);
       if (!good) continue;  // on to the barrier that the other warps wait at
       tmem_fence_after();
-      const int columns = min(p.bt, p.M - at.m0);
+      const int columns = min(at.rows, p.M - at.m0);
       finish_columns<ACT, BF16>(p, f, lanes, at.m0, half * 16, columns, sh.x_scale[buf]);
       tmem_fence_before();
       __syncwarp();

@@ -13,6 +13,7 @@ namespace mgv {
 struct GemmI8Params {
   alignas(64) CUtensorMap w_map;  // weights: boxes of 128 bytes (K) x 128 rows, 128-byte swizzle
   alignas(64) CUtensorMap x_map;  // activations: boxes of 128 bytes x the rows one block copies
+  alignas(64) CUtensorMap x_half_map;  // ... x half of them, for halved tiles
   const float *x_scale;
   const void *w_scale, *bias;
   void *out;
@@ -26,7 +27,8 @@ struct GemmI8Params {
   int split;       // blocks of a cluster that share a tile's K range
   int n_tiles, m_tiles;
   int sums_off;    // split: where the sums arrive in dynamic shared memory; 0: in the ring, once it is free
-  uint32_t idesc;  // instruction descriptor of the matrix instruction
+  int halved;      // pairs: tiles from this one on, in the order of work, come in two halves of their rows
+  uint32_t idesc, half_idesc;  // instruction descriptors of the matrix instruction, for whole and halved tiles
   uint32_t tmem_cols;
 };
 

@@ -254,8 +254,9 @@ def test_every_kernel_and_tiling_gives_the_same_bits(cuda_lib, M, N, K, act, hin
 
 
 def test_more_tiles_than_blocks(cuda_lib):
-    """Every pair of blocks takes several tiles, whose accumulators and ring slots alternate."""
-    for M, N, K in ((2000, 5000, 200), (4096, 8192, 1100)):
+    """Every pair of blocks takes several tiles, whose accumulators and ring slots alternate; the last ones come in
+    halves (of 2000 x 5000 and 1800 x 5000 at 256 rows), some of them with no rows left (of 1800)."""
+    for M, N, K in ((2000, 5000, 200), (1800, 5000, 200), (4096, 8192, 1100)):
         for rows in (64, 256):
             Product(M, N, K, act="gated", seed=7).run(hints=_lib.GEMM_HINT_PAIR | _lib.gemm_hint_rows(rows)).check()
     assert api.device_error_state() == 0
