@@ -332,12 +332,15 @@ mgv_status mgv_gemv_launch_info(const mgv_gemv_args *args, mgv_launch_info *info
  * All calls are asynchronous, allocate nothing, keep no state between calls and may be captured.
  * M = 0 (no rows) is a valid call that launches nothing.  MGV_FLAG_PDL works as in the GEMV: the
  * kernel may start while its predecessor on the stream drains, and touches only norm weights,
- * layer weights, their scales and bias before that predecessor has completed. */
+ * layer weights, their scales and bias before that predecessor has completed.  Those must not be
+ * written by the predecessor, nor by a kernel before it where the predecessor is a GEMV launched
+ * with MGV_FLAG_PDL (which lets its dependents start before its own predecessor has ended; the
+ * kernels here do not).  Outputs must not overlap inputs, except as stated. */
 
 typedef enum mgv_dtype { MGV_DTYPE_F16 = 0, MGV_DTYPE_BF16 = 1, MGV_DTYPE_F32 = 2 } mgv_dtype;
 
-/* x [M][ldx] (dtype: F16 or BF16) -> q int8 [M][ldq], scale fp32 [M].  Any K >= 1 and any leading
- * dimensions >= K; x at its element's alignment, scale 4-byte aligned.  Rows whose addresses are
+/* x [M][ldx] (dtype: F16 or BF16) -> q int8 [M][ldq], scale fp32 [M].  Any K up to 2^30 and any
+ * leading dimensions >= K; x at its element's alignment, scale 4-byte aligned.  Rows whose addresses are
  * multiples of 16 bytes (q: 8) are read and written in vectors.  flags: MGV_FLAG_PDL. */
 mgv_status mgv_quantize_rows(void *q_i8_dev, void *scale_f32_dev, const void *x_dev, int dtype, int64_t M, int32_t K,
                              int64_t ldq, int64_t ldx, int flags, mgv_stream_t s);
@@ -354,8 +357,8 @@ typedef struct mgv_rmsnorm_args {
   int32_t struct_size;
   int32_t dtype;          /* F16 or BF16: x, residual, weight, residual_out                  */
   int32_t flags;          /* MGV_FLAG_PDL                                                     */
-  int32_t K;              /* row length, >= 1                                                 */
-  int64_t M;              /* rows, >= 0                                                       */
+  int32_t K;              /* row length, 1..2^30                                              */
+  int64_t M;              /* rows, 0..2^31-1                                                  */
   const void *x;          /* [M][ldx]                                                         */
   const void *residual;   /* [M][ldr] or NULL                                                 */
   const void *weight;     /* [K]                                                              */

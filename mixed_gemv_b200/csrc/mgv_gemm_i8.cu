@@ -52,14 +52,14 @@ __global__ void __launch_bounds__(kGemmThreads, kGemmBlocksPerSm) gemm_i8_block_
   __syncthreads();
   tmem_fence_after();
   const uint32_t tmem = __shfl_sync(~0u, sh.tmem_base, 0);
-  // only now: a dependent kernel that starts on this SM may hold tensor memory while it waits for this one to end
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int columns = min(p.bt, p.M - m0), quads = (columns + 3) / 4;
   const int mine = p.split > 1 ? (quads - int(rank) + p.split - 1) / p.split : 0;  // column quads this block finishes of a split tile
   if (p.split > 1 && p.sums_off) cluster_arrive<true>();  // this block can be sent to: its barriers are set up
 
   if (warp == 0) {
-    asm volatile("griddepcontrol.wait;\n\tfence.proxy.async.global;" ::: "memory");
+    // A dependent kernel may start only now: behind the wait, so that no kernel runs beside any but its direct
+    // predecessor, and behind the allocation of tensor memory, of which it may hold some while it waits for this one.
+    asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;\n\tfence.proxy.async.global;" ::: "memory");
     if (one) {
       for (int i = 0; i < ahead; ++i)
         box_load(ring + i * slot_bytes + kGemmABytes, &p.x_map, (first + i) * kGemmK, m0, smem_u32(&sh.full[i]));

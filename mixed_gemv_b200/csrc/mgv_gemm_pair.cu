@@ -51,7 +51,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_pair_kernel(const __g
   cluster_sync();
   tmem_fence_after();
   const uint32_t tmem = __shfl_sync(~0u, sh.tmem_base, 0);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (warp == 0) {
     // both blocks' copies count on the first block's barriers; each block waits on its own for a free slot
@@ -64,7 +63,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_pair_kernel(const __g
         box_load_pair(ring + i * slot_bytes, &p.w_map, i * kGemmK, at.n0 + int(rank) * kGemmRows, in_block(smem_u32(&sh.full[i]), 0));
       }
     }
-    asm volatile("griddepcontrol.wait;\n\tfence.proxy.async.global;" ::: "memory");
+    // as in the kernel of single blocks: dependents start behind the wait and the allocation
+    asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;\n\tfence.proxy.async.global;" ::: "memory");
     if (one)
       for (int i = 0; i < ahead; ++i)
         box_load_pair(ring + i * slot_bytes + kGemmABytes, at.rows == p.bt ? &p.x_map : &p.x_half_map, i * kGemmK, at.m0 + int(rank) * at.rows / 2, in_block(smem_u32(&sh.full[i]), 0));

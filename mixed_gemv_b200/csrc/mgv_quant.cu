@@ -10,6 +10,14 @@
 
 namespace mgv {
 
+// Waits for the stream's previous kernel (dependent launches), and only then lets the next one start: so no
+// kernel runs beside any but its direct predecessor, and what it touches before its own wait only has to be
+// older than that.
+__device__ __forceinline__ void wait_for_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 struct RowParams {
   const void *x, *residual, *weight;
   void *residual_out;
@@ -205,7 +213,6 @@ __global__ void __launch_bounds__(WARP_ROW ? 128 : 1024, WARP_ROW ? 6 : 1) rows_
   const int step = WARP_ROW ? 32 : blockDim.x, t = WARP_ROW ? threadIdx.x % 32 : threadIdx.x;
   const int per_block = WARP_ROW ? 4 : 1;
   const int64_t first = int64_t(blockIdx.x) * per_block + (WARP_ROW ? threadIdx.x / 32 : 0), stride = int64_t(gridDim.x) * per_block;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   P w[NORM && kKeepWeight ? NV : 1];
   if (NORM && kKeepWeight) {
 #pragma unroll
@@ -214,7 +221,7 @@ __global__ void __launch_bounds__(WARP_ROW ? 128 : 1024, WARP_ROW ? 6 : 1) rows_
       if (k < p.K) w[i] = load_piece<V>(p.weight, k, p.K - k);
     }
   }
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_previous();
   const bool add = NORM && p.residual;
   // Where registers allow it the next row is on its way while this one is reduced.
   constexpr bool kAhead = V == 8 && !WARP_ROW && NV <= (NORM ? 2 : 4);
@@ -341,8 +348,7 @@ __global__ void __launch_bounds__(kLongThreads, 3) long_rows_kernel(const __grid
   const bool add = NORM && p.residual;
   const T *r = add ? static_cast<const T *>(p.residual) + m * p.ldr : nullptr;
   T *ro = add ? static_cast<T *>(p.residual_out) + m * p.ldro : nullptr;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_previous();
   RowStats s = {0.0f, 0u};
   constexpr int kBatch = 8;  // loads in flight
   for (int k0 = threadIdx.x; k0 < p.K; k0 += kBatch * kLongThreads) {
@@ -418,8 +424,7 @@ __global__ void __launch_bounds__(kBackThreads) back_kernel(const BackParams p) 
   const int64_t chunks = (p.K + width - 1) / width;
   const int64_t m = int64_t(blockIdx.x / chunks) * rows + row;
   const int k = int(blockIdx.x % chunks) * width + (threadIdx.x % p.lanes) * V;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_previous();
   if (m >= p.M || k >= p.K) return;
   const int n = p.K - k;
   const float s = p.scale[m];
@@ -532,7 +537,7 @@ static mgv_status check_rows(const char *what, int dtype, int64_t M, int32_t K, 
   if (dtype != MGV_DTYPE_F16 && dtype != MGV_DTYPE_BF16)
     return fail(MGV_STATUS_UNSUPPORTED, "%s: dtype %d is neither F16 nor BF16", what, dtype);
   if (M < 0 || M > 0x7fffffff) return fail(MGV_STATUS_INVALID_ARGUMENT, "%s: M=%lld outside 0..2^31-1", what, (long long)M);
-  if (K < 1) return fail(MGV_STATUS_INVALID_ARGUMENT, "%s: K=%d must be at least 1", what, K);
+  if (K < 1 || K > (1 << 30)) return fail(MGV_STATUS_INVALID_ARGUMENT, "%s: K=%d outside 1..2^30", what, K);
   if (flags & ~MGV_FLAG_PDL) return fail(MGV_STATUS_INVALID_ARGUMENT, "%s: only MGV_FLAG_PDL applies (flags %d)", what, flags);
   return MGV_STATUS_OK;
 }

@@ -419,6 +419,42 @@ def test_captured_and_replayed_on_new_inputs(cuda_lib):
         layer.check()
 
 
+FIRST_CALL = """
+import torch
+from tests.test_gpu_int8_path import LayerHalf
+layer = LayerHalf(24, 512, 704, torch.float16, seed=3)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    layer.run()
+for _ in range(2):
+    graph.replay()
+torch.cuda.synchronize()
+layer.check()
+print("first call captured")
+"""
+
+
+def test_the_first_run_of_a_process_may_be_captured(cuda_lib):
+    """Plans are made before the capture, nothing has been launched."""
+    import subprocess
+    import sys
+    from tests.conftest import ROOT
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "first call captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_the_call_without_a_plan(cuda_lib):
+    import ctypes as C
+    for M, act in ((0, "none"), (5, "gated"), (300, "silu")):
+        p = Product(M, 130, 200, act=act, bias=True, seed=11)
+        c = api.GemmI8Adaptor._to_c(cuda_lib, p.arguments())
+        assert cuda_lib.mgv_gemm_i8(C.byref(c), None) == Status.OK
+        torch.cuda.synchronize()
+        if M:
+            p.check()
+
+
 def test_run_takes_the_stream_it_is_given(cuda_lib):
     p = Product(9, 96, 256, seed=8)
     op = api.GemmI8Adaptor()

@@ -57,6 +57,7 @@ def test_struct_layouts_match_the_header():
     (dict(M=-1), Status.INVALID_ARGUMENT),
     (dict(M=1 << 31), Status.INVALID_ARGUMENT),
     (dict(K=0), Status.INVALID_ARGUMENT),
+    (dict(K=(1 << 30) + 1, ldx=1 << 31, ldq=1 << 31), Status.INVALID_ARGUMENT),
     (dict(flags=_lib.FLAG_ACT_RELU), Status.INVALID_ARGUMENT),
     (dict(eps=-1e-6), Status.INVALID_ARGUMENT),
     (dict(eps=math.nan), Status.INVALID_ARGUMENT),
