@@ -14,8 +14,8 @@ namespace mgv {
 // the matrix instructions, accumulators are 32-bit integers in tensor memory: lane = feature, column =
 // row of the activations.  With split > 1 every block finishes a share of the columns, out of the sums that all
 // blocks of the cluster send it; integer sums, so the result does not depend on the split.
-constexpr int kQuadBytes = kGemmRows * 16;  // sums of 128 features x 4 columns
-
+// Bound by HBM (weights), and by a call's start, first fetch and exchange, some 3 us, where there is little of those: B200,
+// dependent launches, 1 x 4096 x 4096 5.2 us, 16 x 22016 x 4096 gated 17.5 us (0.79 of the copy bandwidth).
 template <int ACT, bool BF16>
 __global__ void __launch_bounds__(kGemmThreads, kGemmBlocksPerSm) gemm_i8_block_kernel(const __grid_constant__ GemmI8Params p) {
   extern __shared__ uint8_t dynamic[];
@@ -247,15 +247,18 @@ static uint32_t instruction(int rows, int columns) { return 2u << 4 | 1u << 7 | 
 // SM alone takes in 96 bytes a cycle from L2, all SMs together 7500 as single blocks and 9400 as pairs; a slice of
 // 128 K keeps the issuing warp for 330 cycles at least and the matrix unit for the time of its four
 // instructions; HBM delivers 3260 bytes a cycle but for the start and end of a block's row of slices; 16
-// columns of an epilogue take 320 cycles; a split tile's exchange takes 1500 and 45 a column beside the next call's
-// start.  (Of 19 shapes from 1 x 4096 x 4096 to 2048 x 8192 x 28672 -- rows x features x K -- the choice was within
-// 8 % of the best tiling on 17; on 64 x 12288 x 4096 and 131 x 4096 x 11008 it is 14 % off.)
+// columns of an epilogue take 320 cycles; a split tile's exchange takes 1500 and, a column, 30 and
+// 5 for each part beside the next call's start.
+// (Of 20 shapes from 1 x 4096 x 4096 to 4096 x 4096 x 4096 -- rows x features x K -- the choice was within 8 % of the best
+// tiling on 17 and 13 % off at most.)
 constexpr double kSmBytes = 96, kBlockBytes = 7500, kPairBytes = 9400, kHbmBytes = 3260, kIssue = 330, kColumn16 = 320, kStart = 4500;
 
 // chain: of the slices that one block works through; fed: to get all operands from L2 to the SMs
 static double estimate(double chain, double fed, double weights, double tail) {
   return kStart + std::max(std::max(chain, fed), weights / kHbmBytes + 0.4 * chain) + tail;
 }
+
+static double exchange(int bt, int split) { return 1500 + bt * (30.0 + 5 * split); }
 
 static int rounded_columns(int want) { return want == 1 ? 16 : std::min(256, (want + 1) / 2 * 32); }
 
@@ -298,41 +301,41 @@ static void plan_block(GemmI8Plan &pl, int64_t M, int bt, int split, int sms, in
   pl.cluster = split;
   const int64_t at_once = std::max(1, std::min(std::min(kGemmSmShared / (smem + fixed), int(512 / p.tmem_cols)), kGemmBlocksPerSm));
   const double slice = std::max(slot / kSmBytes, 4 * std::max(40.0, bt / 2.0));  // of the SM's time
-  const double tail = split > 1 ? 1500 + 45.0 * bt : kColumn16 * ((bt + 15) / 16);
+  const double tail = split > 1 ? exchange(bt, split) : kColumn16 * ((bt + 15) / 16);
   const int64_t rounds = (on_sm + at_once - 1) / at_once;  // blocks that follow one another: each starts and ends alone
   const double chain = rounds * share * std::max(kIssue, slice) + (rounds - 1) * (2500 + tail);
   const double fed = std::max(double(on_sm) * share * slice, double(grid) * share * slot / kBlockBytes);
   pl.cost = estimate(chain, fed, double(p.N) * p.K, tail);
 }
 
-static void plan_pair(GemmI8Plan &pl, int64_t M, int bt, int sms, int most) {
+static void plan_pair(GemmI8Plan &pl, int64_t M, int bt, int split, int sms, int most) {
   GemmI8Params &p = pl.p;
   p.bt = bt;
-  p.split = 1;
+  p.split = split;
   p.n_tiles = (p.N + 2 * kGemmRows - 1) / (2 * kGemmRows);
   p.m_tiles = int((M + bt - 1) / bt);
   p.tmem_cols = 64;  // two accumulators
   while (int(p.tmem_cols) < 2 * bt) p.tmem_cols *= 2;
   p.idesc = instruction(2 * kGemmRows, bt);
   const int64_t tiles = int64_t(p.n_tiles) * p.m_tiles, pairs = std::min<int64_t>(tiles, sms / 2);
-  const int slices = (p.K + kGemmK - 1) / kGemmK, slot = kGemmABytes + bt / 2 * kGemmK, room = most - int(sizeof(GemmPairShared));
+  const int slices = ((p.K + kGemmK - 1) / kGemmK + split - 1) / split, slot = kGemmABytes + bt / 2 * kGemmK, room = most - int(sizeof(GemmPairShared));
   p.stages = std::min(kGemmMaxStages, (room - kGemmAlign) / slot);
   // the last round's tiles in halves where those are enough for no more than a round of their own
   const int64_t rounds = tiles / pairs, rest = tiles % pairs;
-  const bool halve = rounds > 0 && rest > 0 && 2 * rest <= pairs && bt % 64 == 0;
+  const bool halve = split == 1 && rounds > 0 && rest > 0 && 2 * rest <= pairs && bt % 64 == 0;
   p.halved = int(halve ? tiles - rest : tiles);
   p.half_idesc = instruction(2 * kGemmRows, halve ? bt / 2 : bt);
   pl.pair = 1;
   pl.smem = room;  // one block per SM: it may hold all of the tensor memory
-  pl.grid = int(2 * pairs);
-  pl.cluster = 2;
+  pl.grid = int(2 * std::min<int64_t>(split > 1 ? tiles * split : pairs, 1 << 28));
+  pl.cluster = 2 * split;
   auto round = [&](int rows) {  // a tile's epilogue runs beside the next tile
     const double slice = std::max(std::max((kGemmABytes + rows / 2 * kGemmK) / kSmBytes, kIssue), 2.0 * rows);
     return std::max(slices * slice, kColumn16 * (rows / 16));
   };
-  const double tail = kColumn16 * ((halve ? bt / 2 : bt) / 16);
+  const double tail = split > 1 ? exchange(bt, split) : kColumn16 * ((halve ? bt / 2 : bt) / 16);
   const double chain = rounds * round(bt) + (halve ? round(bt / 2) : rest ? round(bt) : 0);
-  pl.cost = estimate(chain, 2.0 * tiles * slices * slot / kPairBytes, double(p.N) * p.K, tail);
+  pl.cost = estimate(chain, 2.0 * tiles * split * slices * slot / kPairBytes, double(p.N) * p.K, tail);
 }
 
 // The tiling of least estimated cost, of those that the hints leave.
@@ -358,8 +361,13 @@ static mgv_status plan(GemmI8Plan &pl, const mgv_gemm_i8_args *a, int sms, int m
   if (!(a->hints & MGV_GEMM_HINT_BLOCK)) {
     for (int bt = 32; bt <= 256; bt += 32) {
       if (rows ? bt != std::max(32, rounded_columns(rows)) : bt > widest) continue;
-      plan_pair(pl, a->M, bt, sms, most);
-      keep(pl);
+      // pairs share a tile where all clusters fit the GPU at once (of 4 or 8 blocks, 32 or 16 find room in its GPCs)
+      const int64_t tiles = int64_t((a->N + 2 * kGemmRows - 1) / (2 * kGemmRows)) * ((a->M + bt - 1) / bt);
+      for (int split = 1; split <= std::min(4, slices); split *= 2) {
+        if (rows ? split != std::min((a->hints & 7) + 1, slices) : split > 1 && tiles * split > 64) continue;
+        plan_pair(pl, a->M, bt, split, sms, most);
+        keep(pl);
+      }
     }
   }
   if (best.cost == 0) return fail(MGV_STATUS_INVALID_ARGUMENT, "gemm_i8: hints %d leave no kernel", a->hints);

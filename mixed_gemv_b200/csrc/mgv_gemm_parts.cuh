@@ -24,7 +24,7 @@ struct GemmI8Params {
   int wide;        // two neighbouring features can be stored as one aligned word
   int bt;          // activation rows of a tile
   int stages;      // ring slots
-  int split;       // blocks of a cluster that share a tile's K range
+  int split;       // blocks, or pairs of blocks, of a cluster that share a tile's K range
   int n_tiles, m_tiles;
   int sums_off;    // split: where the sums arrive in dynamic shared memory; 0: in the ring, once it is free
   int halved;      // pairs: tiles from this one on, in the order of work, come in two halves of their rows
@@ -53,9 +53,11 @@ struct GemmBlockShared {
 };
 struct GemmPairShared {
   alignas(16) float x_scale[2][256];
-  uint64_t full[kGemmMaxStages], empty[kGemmMaxStages], ready[2], drained[2];
+  uint64_t full[kGemmMaxStages], empty[kGemmMaxStages], ready[2], drained[2], sums;
   uint32_t tmem_base;
 };
+
+constexpr int kQuadBytes = kGemmRows * 16;  // sums of 128 features x 4 columns
 
 enum { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGated = 3 };
 
@@ -188,10 +190,11 @@ __device__ __forceinline__ uint32_t in_block(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void arrive_in_block(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// Arrives at the barrier `bar` of both blocks of a pair when the matrix instructions issued so far have completed.
-__device__ __forceinline__ void commit_pair(uint32_t bar) {
+// Arrives at the barrier `bar` of both blocks of a pair, the first of which has rank `lead`, when the matrix
+// instructions issued so far have completed.
+__device__ __forceinline__ void commit_pair(uint32_t bar, uint32_t lead) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-               "h"(uint16_t(3))
+               "h"(uint16_t(3u << lead))
                : "memory");
 }
 // 16 bytes into the shared memory of a block of the cluster, counted on that block's barrier `bar`

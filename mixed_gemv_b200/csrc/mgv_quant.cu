@@ -202,7 +202,8 @@ constexpr float kLeft = -1.0f;
 // quantisation, and one reduction serves both: with y = h w r, r = 1 / sqrt(mean + eps), the scale is
 // r max|h w| / 127 and q = h w 127 / max|h w|, in which r does not occur.  The sum of squares, the
 // largest value and the scale are fp32.  A block takes a row (a warp, for short rows) with NV pieces of V
-// values to a thread, then the next one; the norm's weights stay in registers over its rows.
+// values to a thread, then the next one; the norm's weights stay in registers over its rows where there is room.
+// Bound by HBM: B200, 4096 x 8192 bf16 with residual 37.8 us (6.2 TB/s, 0.95 of the copy bandwidth), without norm 16.5 us.
 template <typename T, bool NORM, int V, int NV, bool WARP_ROW>
 __global__ void __launch_bounds__(WARP_ROW ? 128 : 1024, WARP_ROW ? 6 : 1) rows_kernel(const __grid_constant__ RowParams p) {
   constexpr bool kKeepWeight = NV <= 2 || (V == 1 && NV == 8);
@@ -416,7 +417,7 @@ struct BackParams {
 constexpr int kBackThreads = 256;
 
 // 16 neighbouring values to a thread (V = 16), or eight that are p.lanes apart (V = 1); a block takes
-// kBackThreads / lanes rows.
+// kBackThreads / lanes rows.  Bound by HBM: B200, 4096 x 8192 bf16 16.6 us (6.1 TB/s).
 template <typename T, int V>
 __global__ void __launch_bounds__(kBackThreads) back_kernel(const BackParams p) {
   constexpr int kEach = V == 1 ? 8 : V;

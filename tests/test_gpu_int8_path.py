@@ -241,7 +241,7 @@ def test_gemm(cuda_lib, M, N, K, act):
 
 
 PATHS = [_lib.GEMM_HINT_BLOCK | _lib.gemm_hint_split(s) | _lib.gemm_hint_rows(r) for s in (1, 2, 4, 8) for r in (16, 96, 256)] + \
-        [_lib.GEMM_HINT_PAIR | _lib.gemm_hint_rows(r) for r in (32, 96, 160, 256)]
+        [_lib.GEMM_HINT_PAIR | _lib.gemm_hint_split(s) | _lib.gemm_hint_rows(r) for s in (1, 2, 4) for r in (32, 96, 160, 256)]
 
 
 @pytest.mark.parametrize("hints", PATHS)
