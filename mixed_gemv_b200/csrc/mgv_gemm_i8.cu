@@ -364,7 +364,8 @@ static mgv_status plan(GemmI8Plan &pl, const mgv_gemm_i8_args *a, int sms, int m
       // pairs share a tile where all clusters fit the GPU at once (of 4 or 8 blocks, 32 or 16 find room in its GPCs)
       const int64_t tiles = int64_t((a->N + 2 * kGemmRows - 1) / (2 * kGemmRows)) * ((a->M + bt - 1) / bt);
       for (int split = 1; split <= std::min(4, slices); split *= 2) {
-        if (rows ? split != std::min((a->hints & 7) + 1, slices) : split > 1 && tiles * split > 64) continue;
+        if (rows ? 2 * split <= std::min((a->hints & 7) + 1, std::min(4, slices)) : split > 1 && tiles * split > 64) continue;
+        if (rows && split > (a->hints & 7) + 1) break;
         plan_pair(pl, a->M, bt, split, sms, most);
         keep(pl);
       }

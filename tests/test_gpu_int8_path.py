@@ -39,7 +39,9 @@ def _check_quantised(q, scale, y, top_slack, scale_tol):
 
 
 SHAPES = [(1, 1), (1, 7), (3, 8), (2, 64), (5, 100), (64, 1024), (7, 1031), (4, 4096), (3, 5001), (2, 8192), (9, 11008),
-          (3, 16392), (2, 28672), (1, 65536), (2, 65543), (2, 70000), (1500, 256), (1000, 24)]
+          (3, 16392), (2, 28672), (1, 65536), (2, 65543), (2, 70000), (1500, 256), (1000, 24),
+          # more rows than blocks at a time
+          (12000, 136), (3000, 1031), (1400, 4096), (700, 8200), (500, 9001), (400, 28680)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -113,6 +115,53 @@ def test_rows_without_and_beyond_numbers(cuda_lib, K, dtype):
         # a subnormal fp32 scale is a whole number of 2^-149, half a step off at most (in _check_quantised);
         # the norm's fp32 statistics as in test_rmsnorm
         _check_quantised(q[good], s[good], y, 4 * U, (2 if not norm else 150) * U)
+
+
+@pytest.mark.parametrize("K", [136, 1031, 4096, 8200])
+def test_wild_rows_among_many(cuda_lib, K):
+    """Rows that need double precision, or hold no numbers, between ordinary ones of the same block."""
+    M, dtype = 3000, torch.bfloat16
+    g = _gen(K)
+    x, r = torch.randn(M, K, generator=g, device="cuda").to(dtype), torch.randn(M, K, generator=g, device="cuda").to(dtype)
+    for start, factor in ((0, 1e-25), (1, 1e25), (2, 0.0)):
+        x[start::7] *= factor
+        r[start::7] *= factor
+    x[3::700, K // 3] = float("inf")
+    x[4::700, K - 1] = float("nan")
+    w = (1 + 0.2 * torch.randn(K, generator=g, device="cuda")).to(dtype)
+    q, s, ro = torch.empty(M, K, dtype=torch.int8, device="cuda"), torch.empty(M, device="cuda"), torch.empty_like(x)
+    api.RmsNormQuantizer()(api.RmsNormQuantizeArguments(x=x, weight=w, q=q, scale=s, residual=r, residual_out=ro, eps=0.0))
+    h, y = _norm_reference(x, r, w, 0.0)
+    assert torch.equal(torch.nan_to_num(ro), torch.nan_to_num(h))
+    bad = torch.zeros(M, dtype=torch.bool, device="cuda")
+    bad[3::700] = bad[4::700] = True
+    assert bool(s[bad].isnan().all()) and not bool(q[bad].any()) and not bool(s[~bad].isnan().any())
+    zero = h.float().abs().amax(dim=1) == 0
+    assert not bool(q[zero].any()) and not bool(s[zero].any())
+    y[zero] = 0
+    _check_quantised(q[~bad], s[~bad], y[~bad], 4 * U, 154 * U)
+
+
+def test_offsets_beyond_32_bits(cuda_lib):
+    """Three rows, gigabytes apart."""
+    M, K, N, far = 3, 520, 264, 1_500_000_016
+    x, _ = _strided(M, K, torch.float16, far)
+    x.copy_(torch.randn(M, K, generator=_gen(1), device="cuda"))
+    q, _ = _strided(M, K, torch.int8, 2 * far)
+    s, w = torch.empty(M, device="cuda"), torch.ones(K, dtype=torch.float16, device="cuda")
+    api.RowQuantizer()(api.RowQuantizeArguments(x=x, q=q, scale=s))
+    _check_quantised(q, s, x.double(), 3 * U, 2 * U)
+    want = x.clone() + x.clone()
+    api.RmsNormQuantizer()(api.RmsNormQuantizeArguments(x=x, weight=w, q=q, scale=s, residual=x, residual_out=x))
+    assert torch.equal(x, want)
+    _check_quantised(q, s, _norm_reference(want, None, w, float(torch.tensor(1e-5)))[1], 4 * U, 154 * U)
+    api.RowDequantizer()(api.RowDequantizeArguments(q=q, scale=s, out=x))
+    back = q.double() * s.double()[:, None]
+    assert torch.all((x.double() - back).abs() <= (2.0 ** -11 + 2 * U) * back.abs() + 2.0 ** -25)
+    p = Product(M, N, K, bias=True)
+    p.out, _ = _strided(M, N, torch.float16, far)
+    p.x, p.xs = q, s
+    p.run().check()
 
 
 # ---- norm ---------------------------------------------------------------------------------------
@@ -274,6 +323,13 @@ def test_gemm_types_and_activations(cuda_lib, M, act, scales, dtype):
 @pytest.mark.parametrize("M, N, ldd, offset", [(5, 256, 300, 0), (40, 256, 257, 1), (300, 512, 520, 8), (300, 512, 515, 3), (600, 130, 131, 2)])
 def test_gemm_strides(cuda_lib, M, N, ldd, offset, act):
     p = Product(M, N, 200, act=act, pad=48, ldd=ldd, out_offset=offset, seed=9).run().check()
+    p.check_surroundings()
+
+
+@pytest.mark.parametrize("M", [3, 40, 300])
+def test_gemm_odd_features_in_even_rows(cuda_lib, M):
+    """The last feature stands alone in rows whose others are stored two at a time."""
+    p = Product(M, 517, 300, bias=True, ldd=520, seed=12).run().check()
     p.check_surroundings()
 
 
