@@ -416,46 +416,52 @@ struct BackParams {
 
 constexpr int kBackThreads = 256;
 
-// 16 neighbouring values to a thread (V = 16), or eight that are p.lanes apart (V = 1); a block takes
-// kBackThreads / lanes rows.  Bound by HBM: B200, 4096 x 8192 bf16 16.6 us (6.1 TB/s).
+// Four int8 values of a word, as floats times s: q + 128 in the mantissa of 2^23 is exact, without a
+// conversion instruction.
+__device__ __forceinline__ float4 scaled4(uint32_t word, float s) {
+  const uint32_t u = word ^ 0x80808080u;
+  return make_float4((__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540)) - 8388736.0f) * s,
+                     (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7541)) - 8388736.0f) * s,
+                     (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7542)) - 8388736.0f) * s,
+                     (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7543)) - 8388736.0f) * s);
+}
+template <typename T>
+__device__ __forceinline__ uint4 scaled8(uint32_t lo, uint32_t hi, float s) {
+  const float4 f = scaled4(lo, s), g = scaled4(hi, s);
+  return make_uint4(pack2<T>(f.x, f.y), pack2<T>(f.z, f.w), pack2<T>(g.x, g.y), pack2<T>(g.z, g.w));
+}
+
+// A block takes kBackThreads / lanes rows, a thread 16 neighbouring values of rows at 16-byte addresses (V = 16).
+// Of other rows it takes the eight that one aligned 16-byte piece of the output holds (V = 8), out of the three words
+// around their bytes; pieces that reach beyond the row go value by value.  Bound by HBM: B200, 4096 x 8192 bf16
+// 16.6 us (6.1 TB/s).
 template <typename T, int V>
 __global__ void __launch_bounds__(kBackThreads) back_kernel(const BackParams p) {
-  constexpr int kEach = V == 1 ? 8 : V;
-  const int rows = kBackThreads / p.lanes, row = threadIdx.x / p.lanes, width = p.lanes * kEach;
-  const int64_t chunks = (p.K + width - 1) / width;
-  const int64_t m = int64_t(blockIdx.x / chunks) * rows + row;
-  const int k = int(blockIdx.x % chunks) * width + (threadIdx.x % p.lanes) * V;
+  const int rows = kBackThreads / p.lanes, row = threadIdx.x / p.lanes, width = p.lanes * V;
+  const uint32_t chunks = uint32_t((int64_t(p.K) + (V == 8 ? 7 : 0) + width - 1) / width);
+  const uint32_t group = blockIdx.x / chunks, chunk = blockIdx.x - group * chunks;
+  const int64_t m = int64_t(group) * rows + row;
+  T *out = static_cast<T *>(p.out) + m * p.ldo;
+  const int8_t *q = p.q + m * p.ldq;
+  int k = int(chunk) * width + (threadIdx.x % p.lanes) * V;
+  if (V == 8) k -= int(reinterpret_cast<uintptr_t>(out) / 2 % 8);
   wait_for_previous();
   if (m >= p.M || k >= p.K) return;
-  const int n = p.K - k;
   const float s = p.scale[m];
-  T *out = static_cast<T *>(p.out) + m * p.ldo + k;
-  const int8_t *q = p.q + m * p.ldq + k;
-  if (V == 1) {
-    float f[kEach];
-#pragma unroll
-    for (int j = 0; j < kEach; ++j)
-      if (j * p.lanes < n) f[j] = float(q[j * p.lanes]);
-#pragma unroll
-    for (int j = 0; j < kEach; ++j)
-      if (j * p.lanes < n) out[j * p.lanes] = from_f<T>(f[j] * s);
-  } else if (n >= V) {
-    const uint4 b = *reinterpret_cast<const uint4 *>(q);
-    const uint32_t word[4] = {b.x, b.y, b.z, b.w};
-    uint32_t o[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float f[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)  // q + 128 in the mantissa of 2^23: exact, without a conversion instruction
-        f[j] = (__uint_as_float(__byte_perm(word[i] ^ 0x80808080u, 0x4b000000u, 0x7540 + j)) - 8388736.0f) * s;
-      o[2 * i] = pack2<T>(f[0], f[1]);
-      o[2 * i + 1] = pack2<T>(f[2], f[3]);
+  if (k >= 0 && k + V <= p.K) {
+    if constexpr (V == 16) {
+      const uint4 b = *reinterpret_cast<const uint4 *>(q + k);
+      reinterpret_cast<uint4 *>(out + k)[0] = scaled8<T>(b.x, b.y, s);
+      reinterpret_cast<uint4 *>(out + k)[1] = scaled8<T>(b.z, b.w, s);
+    } else {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(q + k);
+      const uint32_t *words = reinterpret_cast<const uint32_t *>(at & ~uintptr_t(3));
+      const int shift = int(at & 3) * 8;
+      const uint32_t w0 = words[0], w1 = words[1], w2 = shift ? words[2] : 0;
+      *reinterpret_cast<uint4 *>(out + k) = scaled8<T>(__funnelshift_r(w0, w1, shift), __funnelshift_r(w1, w2, shift), s);
     }
-    reinterpret_cast<uint4 *>(out)[0] = make_uint4(o[0], o[1], o[2], o[3]);
-    reinterpret_cast<uint4 *>(out)[1] = make_uint4(o[4], o[5], o[6], o[7]);
   } else {
-    for (int j = 0; j < n; ++j) out[j] = from_f<T>(float(q[j]) * s);
+    for (int j = max(0, -k); j < V && k + j < p.K; ++j) out[k + j] = from_f<T>(float(q[k + j]) * s);
   }
 }
 
@@ -526,11 +532,12 @@ template <typename T>
 static mgv_status dequantise(BackParams p, int flags, cudaStream_t s) {
   const bool wide = aligned_rows(p.q, p.ldq, 1, p.M, 16) && aligned_rows(p.out, p.ldo, 2, p.M, 16);
   const int v = wide ? 16 : 8;
+  const int64_t reach = int64_t(p.K) + (wide ? 0 : 7);  // a row may begin inside its first piece
   p.lanes = 1;
-  while (p.lanes < kBackThreads && p.lanes * v < p.K) p.lanes *= 2;
+  while (p.lanes < kBackThreads && p.lanes * v < reach) p.lanes *= 2;
   const int rows = kBackThreads / p.lanes;
-  const int64_t grid = (p.M + rows - 1) / rows * ((p.K + p.lanes * v - 1) / (p.lanes * v));
-  return wide ? launch_rows(back_kernel<T, 16>, grid, kBackThreads, flags, s, p) : launch_rows(back_kernel<T, 1>, grid, kBackThreads, flags, s, p);
+  const int64_t grid = (p.M + rows - 1) / rows * ((reach + p.lanes * v - 1) / (p.lanes * v));
+  return wide ? launch_rows(back_kernel<T, 16>, grid, kBackThreads, flags, s, p) : launch_rows(back_kernel<T, 8>, grid, kBackThreads, flags, s, p);
 }
 
 // What the three entry points check alike; `what` names the call in the message.
