@@ -191,6 +191,31 @@ def test_rmsnorm(cuda_lib, M, K, with_residual, dtype):
     _check_quantised(q, s, y, 4 * U, 154 * U)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K", [3, 40, 263, 1031, 4100, 9001, 16377])
+@pytest.mark.parametrize("offsets", [(0, 1, 2, 3, 1), (1, 1, 1, 0, 0), (5, 3, 5, 2, 7), (7, 0, 3, 5, 2)])
+def test_norm_of_operands_apart(cuda_lib, K, offsets, dtype):
+    """x, residual, residual_out, weight and q each at an address and a distance of rows of its own; what lies around
+    the outputs is left as it was."""
+    M, g = 7, _gen(K)
+    ox, orr, oro, ow, oq = offsets
+    x, _ = _strided(M, K, dtype, K + 1, ox)
+    r, _ = _strided(M, K, dtype, K + 3, orr)
+    ro, roflat = _strided(M, K, dtype, K + 2, oro, fill=5.0)
+    q, qflat = _strided(M, K, torch.int8, K + 5, oq, fill=77)
+    w = torch.empty(K + 8, dtype=dtype, device="cuda")[ow:ow + K] if ow else torch.empty(K, dtype=dtype, device="cuda")
+    for a in (x, r, w):
+        a.copy_(torch.randn(a.shape, generator=g, device="cuda"))
+    s = torch.empty(M, device="cuda")
+    api.RmsNormQuantizer()(api.RmsNormQuantizeArguments(x=x, weight=w, q=q, scale=s, residual=r, residual_out=ro))
+    h, y = _norm_reference(x, r, w, float(torch.tensor(1e-5)))
+    assert torch.equal(ro, h)
+    _check_quantised(q, s, y, 4 * U, 154 * U)
+    ro.fill_(5.0)
+    q.fill_(77)
+    assert bool((roflat == 5.0).all()) and bool((qflat == 77).all())
+
+
 def test_rmsnorm_eps_matters_and_large_values_do_not_overflow(cuda_lib):
     K = 4096
     x = torch.randn(4, K, generator=_gen(1), device="cuda")
