@@ -381,7 +381,9 @@ mgv_status mgv_rmsnorm_quantize(const mgv_rmsnorm_args *args, mgv_stream_t s);
  * epilogue computes in fp32 and rounds once.  weights are NOT preprocessed: the int8 matrix as
  * mgv_preprocess_weights takes it with MGV_LAYOUT_COLUMN_MAJOR, K contiguous for each feature.
  * A layer that also decodes through mgv_gemv keeps both forms (the GEMV's interleave follows the
- * reference and is not one the tensor cores' 8-bit operands can be copied from).  flags:
+ * reference and is not one the tensor cores' 8-bit operands can be copied from).  Waits inside
+ * the kernels are bounded (about one second); one that gives up sets the device error word
+ * (mgv_device_error_state) and leaves outputs unwritten.  flags:
  * MGV_FLAG_ACT_RELU or MGV_FLAG_ACT_SILU (not both); MGV_FLAG_GATED_SILU as in the GEMV: rows 2i
  * and 2i+1 of weights, scales and bias are gate and up, out has N/2 features; MGV_FLAG_PDL. */
 typedef struct mgv_gemm_i8_args {
