@@ -174,7 +174,8 @@ __device__ __forceinline__ bool row_is_tame(const RowParams &p, const RowStats &
 template <bool NORM>
 __device__ __forceinline__ void row_factors(const RowStats &s, float mean, float &scale, float &inv) {
   const float top = __uint_as_float(s.top);
-  scale = (NORM ? top * rsqrtf(mean) : top) / 127.0f;
+  scale = top / 127.0f;  // first: the largest y itself may be beyond fp32
+  if (NORM) scale *= rsqrtf(mean);
   inv = s.top ? 127.0f / top : 0.0f;
 }
 __device__ __forceinline__ RowStats warp_stats(RowStats s) {

@@ -231,6 +231,18 @@ def test_rmsnorm_eps_matters_and_large_values_do_not_overflow(cuda_lib):
         _check_quantised(q, s, y, 4 * U, 154 * U)
 
 
+@pytest.mark.parametrize("K", [4096, 5001])
+def test_rmsnorm_of_one_value_and_the_largest_weights(cuda_lib, K):
+    """y is beyond fp32, its scale is not."""
+    x = torch.zeros(2, K, dtype=torch.bfloat16, device="cuda")
+    x[:, K // 2] = 1
+    w = torch.full((K,), 3e38, dtype=torch.bfloat16, device="cuda")
+    q, s = torch.empty(2, K, dtype=torch.int8, device="cuda"), torch.empty(2, device="cuda")
+    api.RmsNormQuantizer()(api.RmsNormQuantizeArguments(x=x, weight=w, q=q, scale=s, eps=0.0))
+    assert bool(s.isfinite().all())
+    _check_quantised(q, s, _norm_reference(x, None, w, 0.0)[1], 4 * U, 154 * U)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("K, ld", [(512, 520), (5001, 5003), (4096, 4096), (70000, 70000)])
 @pytest.mark.parametrize("onto", ["residual", "x"])
