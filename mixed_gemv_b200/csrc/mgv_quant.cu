@@ -147,7 +147,6 @@ __device__ __noinline__ void row_in_double(const RowParams &p, int64_t m, int t,
     top = block_reduce_double(top, true, buf);
     bad = block_reduce_double(bad, true, buf);
   }
-  const double inv = top > 0 ? 127.0 / top : 0.0;
   if (t == 0) {
     double s = top / 127.0;
     if (NORM && top > 0) s /= sqrt(ss / p.K + double(p.eps));
@@ -155,7 +154,7 @@ __device__ __noinline__ void row_in_double(const RowParams &p, int64_t m, int t,
   }
   for (int k = t; k < p.K; k += step) {
     const double v = to_f(h[k]), y = NORM ? v * double(to_f(w[k])) : v;
-    q[k] = bad != 0 ? 0 : int8_t(rint(y * inv));
+    q[k] = bad != 0 || top == 0 ? 0 : int8_t(rint(y * 127.0 / top));  // y has 24 bits at most: the product is exact, and so is a tie
   }
 }
 
@@ -171,13 +170,26 @@ __device__ __forceinline__ bool row_is_tame(const RowParams &p, const RowStats &
   const bool sum_ok = !NORM || (mean >= 1e-30f && mean <= FLT_MAX);
   return sum_ok && (s.top == 0 || (s.top >= __float_as_uint(1e-30f) && s.top < 0x7f800000u));
 }
+struct RowFactors {
+  float scale, inv, rest;  // inv + rest = 127 / top to 40 bits and more (28 for a top near fp32's largest, where rest is subnormal)
+};
 template <bool NORM>
-__device__ __forceinline__ void row_factors(const RowStats &s, float mean, float &scale, float &inv) {
+__device__ __forceinline__ RowFactors row_factors(const RowStats &s, float mean) {
   const float top = __uint_as_float(s.top);
-  scale = top / 127.0f;  // first: the largest y itself may be beyond fp32
-  if (NORM) scale *= rsqrtf(mean);
-  inv = s.top ? 127.0f / top : 0.0f;
+  RowFactors f;
+  f.scale = top / 127.0f;  // first: the largest y itself may be beyond fp32
+  if (NORM) f.scale *= rsqrtf(mean);
+  f.inv = s.top ? 127.0f / top : 0.0f;
+  f.rest = fmaf(-f.inv, top, 127.0f) * (f.inv / 127.0f);
+  return f;
 }
+// y * 127 / top as an integer in the low bits of the result, ties to even.  The quotient is rounded to fp32 once, out of
+// more bits than fp32 has, and then to the integer.  A tie is a number of fp32, so the first rounding returns it, and leaves
+// the second to decide.  A quotient that is none stays off it: with a y of b bits it is 1 / (254 * 2^b) of itself away from
+// the next tie, more than half a step of fp32 for b <= 16.  (Only the products of fp16 norms have more bits, up to 22: of
+// those some within 2^-24 of a tie are taken for one.)  With the one product y * inv its error decided at a tie.  Two
+// instructions a value; they do not show beside the memory traffic.
+__device__ __forceinline__ float level(float y, const RowFactors &f) { return fmaf(y, f.inv, y * f.rest) + kRoundMagic; }
 __device__ __forceinline__ RowStats warp_stats(RowStats s) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) s.ss += __shfl_xor_sync(~0u, s.ss, o);
@@ -297,9 +309,8 @@ __global__ void __launch_bounds__(WARP_ROW ? 128 : 1024, WARP_ROW ? 6 : 1) rows_
       if (t == 0) p.scale[m] = kLeft;
       left = true;
     }
-    float scale, inv;
-    row_factors<NORM>(s, mean, scale, inv);
-    if (t == 0 && tame) p.scale[m] = scale;
+    const RowFactors f = row_factors<NORM>(s, mean);
+    if (t == 0 && tame) p.scale[m] = f.scale;
     int8_t *q = p.q + m * p.ldq;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -315,7 +326,7 @@ __global__ void __launch_bounds__(WARP_ROW ? 128 : 1024, WARP_ROW ? 6 : 1) rows_
             const float2 g = unpack2<T>(wi.u[j]);
             v = make_float2(v.x * g.x, v.y * g.y);
           }
-          y[j] = make_float2(fmaf(v.x, inv, kRoundMagic), fmaf(v.y, inv, kRoundMagic));
+          y[j] = make_float2(level(v.x, f), level(v.y, f));
         }
         if constexpr (V == 8) {
           const uint2 o = make_uint2(pack4(y[0].x, y[0].y, y[1].x, y[1].y), pack4(y[2].x, y[2].y, y[3].x, y[3].y));
@@ -381,9 +392,8 @@ __global__ void __launch_bounds__(kLongThreads, 3) long_rows_kernel(const __grid
     row_in_double<T, NORM, false>(p, m, threadIdx.x, kLongThreads, buf);
     return;
   }
-  float scale, inv;
-  row_factors<NORM>(s, mean, scale, inv);
-  if (threadIdx.x == 0) p.scale[m] = scale;
+  const RowFactors f = row_factors<NORM>(s, mean);
+  if (threadIdx.x == 0) p.scale[m] = f.scale;
   const T *again = add ? ro : x;  // every thread reads back what it wrote
   int8_t *q = p.q + m * p.ldq;
   for (int k0 = threadIdx.x; k0 < p.K; k0 += kBatch * kLongThreads) {
@@ -401,7 +411,7 @@ __global__ void __launch_bounds__(kLongThreads, 3) long_rows_kernel(const __grid
       const int k = k0 + j * kLongThreads;
       if (k < p.K) {
         const float v = to_f(h[j]);
-        q[k] = int8_t(__float_as_uint(fmaf(NORM ? v * to_f(g[j]) : v, inv, kRoundMagic)) & 0xff);
+        q[k] = int8_t(__float_as_uint(level(NORM ? v * to_f(g[j]) : v, f)) & 0xff);
       }
     }
   }

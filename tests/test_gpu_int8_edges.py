@@ -1,0 +1,69 @@
+"""GPU tests of the 8-bit activation path at its edges: ties of the quantisation."""
+import pytest
+import torch
+
+from mixed_gemv_b200 import api
+from tests.test_gpu_int8_path import _gen
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- ties of the quantisation -------------------------------------------------------------------
+
+def _quotient(y):
+    """y * 127 / max|y| of rows of up to 24-bit values.  The product has 31 bits, so it is exact; a tie, which has eight, is
+    a number that the division returns exactly, and any other quotient of such numbers is further from a tie than it errs."""
+    return y * 127 / y.abs().amax(dim=1, keepdim=True)
+
+
+def _ties(quotient):
+    twice = quotient * 2
+    return (twice == twice.round()) & (twice.round() % 2 != 0)
+
+
+# rows to a warp, one and two and four pieces a thread, value by value in registers, in two passes
+TIE_SHAPES = [(1500, 256), (3, 4096), (400, 4096), (3, 11008), (400, 11008), (300, 1031), (5, 5001), (400, 5001), (2, 70000), (2, 65536)]
+
+
+def _tie_rows(M, K, dtype, kind, seed):
+    g = _gen(seed)
+    if kind == "normal":
+        return torch.randn(M, K, generator=g, device="cuda").to(dtype)
+    # a grid of up to 122 steps to a row's largest value, an even number of steps: half of it is a tie
+    top = torch.randint(23, 62, (M, 1), generator=g, device="cuda") * 2
+    x = (torch.rand(M, K, generator=g, device="cuda") * 2 - 1).mul(top).round()
+    x[:, K // 2 : K // 2 + 1] = top
+    x[:, K - 1:] = -top / 2
+    return (x * (2.0 ** -120 if kind == "tiny grid" else 1)).to(dtype)  # tiny: statistics below fp32's, rows done in double precision
+
+
+@pytest.mark.parametrize("dtype, kind", [(torch.float16, "normal"), (torch.bfloat16, "normal"), (torch.float16, "grid"),
+                                         (torch.bfloat16, "grid"), (torch.bfloat16, "tiny grid")])
+@pytest.mark.parametrize("M, K", TIE_SHAPES)
+def test_ties_go_to_the_even_integer(cuda_lib, M, K, dtype, kind):
+    x = _tie_rows(M, K, dtype, kind, seed=K)
+    q, s = torch.full((M, K), 99, dtype=torch.int8, device="cuda"), torch.empty(M, device="cuda")
+    api.RowQuantizer()(api.RowQuantizeArguments(x=x, q=q, scale=s))
+    quotient = _quotient(x.double())
+    assert kind == "normal" or bool(_ties(quotient).any(dim=1).all())
+    # With a value of up to 11 bits a quotient that is no tie is at least 1 / (254 * 2^11) > 2^-19 of itself away from one:
+    # fp32 arithmetic to 2^-24 has no other answer than the nearest integer.
+    assert torch.equal(q.double(), quotient.round())
+
+
+@pytest.mark.parametrize("dtype, kind", [(torch.float16, "normal"), (torch.bfloat16, "normal"), (torch.float16, "grid"),
+                                         (torch.bfloat16, "grid"), (torch.bfloat16, "tiny grid")])
+@pytest.mark.parametrize("M, K", TIE_SHAPES)
+def test_ties_behind_the_norm(cuda_lib, M, K, dtype, kind):
+    """y = h w / rms: its ties are those of h w, in which the root does not occur."""
+    x = _tie_rows(M, K, dtype, kind, seed=K + 1)
+    w = (torch.randint(4, 13, (K,), generator=_gen(K), device="cuda") / 8).to(dtype)
+    q, s = torch.full((M, K), 99, dtype=torch.int8, device="cuda"), torch.empty(M, device="cuda")
+    api.RmsNormQuantizer()(api.RmsNormQuantizeArguments(x=x, weight=w, q=q, scale=s, eps=0.0))
+    quotient = _quotient(x.double() * w.double())
+    ties, want = _ties(quotient), quotient.round()
+    assert kind == "normal" or bool(ties.any())
+    assert torch.equal(q.double()[ties], want[ties])
+    # Products of the weights here (4 bits) and x have up to 15 bits: no quotient but a tie is within 1 / (254 * 2^15) > 2^-23
+    # of itself of one.
+    assert torch.equal(q.double(), want)
