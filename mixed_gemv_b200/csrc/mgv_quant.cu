@@ -351,7 +351,10 @@ __global__ void __launch_bounds__(WARP_ROW ? 128 : 1024, WARP_ROW ? 6 : 1) rows_
     if (*static_cast<volatile float *>(p.scale + m) == kLeft) row_in_double<T, NORM, WARP_ROW>(p, m, t, step, buf);
 }
 
-// Rows too long for registers: a block per row, value by value, in two passes over it.
+// Rows too long for registers: a block per row, value by value, in two passes over it.  A thread adds the squares of up to
+// kRun / kLongThreads = 96 of its values, and these sums with what each addition loses carried along (Kahan's sum): the error
+// stays below 100 steps of fp32 and 10 more in the block's reduction, however long the row.  One running sum of a thread's
+// K / 512 values was off by 1e-3 at K = 2^26.
 template <typename T, bool NORM>
 __global__ void __launch_bounds__(kLongThreads, 3) long_rows_kernel(const __grid_constant__ RowParams p) {
   __shared__ RowStats stats[32];
@@ -363,7 +366,15 @@ __global__ void __launch_bounds__(kLongThreads, 3) long_rows_kernel(const __grid
   T *ro = add ? static_cast<T *>(p.residual_out) + m * p.ldro : nullptr;
   wait_for_previous();
   RowStats s = {0.0f, 0u};
-  constexpr int kBatch = 8;  // loads in flight
+  float ss = 0, lost = 0;
+  constexpr int kBatch = 6;  // loads in flight of each operand (eight with a residual spill: 16.3 us for 12.9, 1000 x 5001)
+  constexpr int kRun = 16 * kBatch * kLongThreads;
+  auto fold = [&] {
+    const float add_now = ss - lost, sum = s.ss + add_now;
+    lost = (sum - s.ss) - add_now;
+    s.ss = sum;
+    ss = 0;
+  };
   for (int k0 = threadIdx.x; k0 < p.K; k0 += kBatch * kLongThreads) {
     T h[kBatch], a[kBatch], g[kBatch];
 #pragma unroll
@@ -381,11 +392,13 @@ __global__ void __launch_bounds__(kLongThreads, 3) long_rows_kernel(const __grid
       if (k < p.K) {
         if (add) ro[k] = h[j] = from_f<T>(to_f(h[j]) + to_f(a[j]));
         const float v = to_f(h[j]), y = NORM ? v * to_f(g[j]) : v;
-        if (NORM) s.ss = fmaf(v, v, s.ss);
+        if (NORM) ss = fmaf(v, v, ss);
         s.top = max(s.top, __float_as_uint(y) & 0x7fffffffu);
       }
     }
+    if (NORM && (k0 + kBatch * kLongThreads) % kRun < kLongThreads) fold();
   }
+  if (NORM) fold();
   s = block_stats(s, stats);
   const float mean = s.ss / float(p.K) + p.eps;
   if (!row_is_tame<NORM>(p, s, mean)) {

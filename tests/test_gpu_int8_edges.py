@@ -1,9 +1,9 @@
-"""GPU tests of the 8-bit activation path at its edges: ties of the quantisation."""
+"""GPU tests of the 8-bit activation path at its edges: ties of the quantisation, long rows."""
 import pytest
 import torch
 
 from mixed_gemv_b200 import api
-from tests.test_gpu_int8_path import _gen
+from tests.test_gpu_int8_path import U, _check_quantised, _gen, _norm_reference
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +67,17 @@ def test_ties_behind_the_norm(cuda_lib, M, K, dtype, kind):
     # Products of the weights here (4 bits) and x have up to 15 bits: no quotient but a tie is within 1 / (254 * 2^15) > 2^-23
     # of itself of one.
     assert torch.equal(q.double(), want)
+
+
+# ---- rows of many values ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("K", [1 << 24, (1 << 26) + 3])
+def test_norm_of_a_long_row_of_one_value(cuda_lib, K):
+    """Equal squares: a sum that loses part of each of them is off by as much in all."""
+    x = torch.full((1, K), 0.7, dtype=torch.float16, device="cuda")
+    x[0, K // 3] = -1.5
+    w = torch.ones(K, dtype=torch.float16, device="cuda")
+    q, s = torch.empty(1, K, dtype=torch.int8, device="cuda"), torch.empty(1, device="cuda")
+    api.RmsNormQuantizer()(api.RmsNormQuantizeArguments(x=x, weight=w, q=q, scale=s, eps=0.0))
+    # the scale as in test_rmsnorm of the shorter rows
+    _check_quantised(q, s, _norm_reference(x, None, w, 0.0)[1], 4 * U, 154 * U)
