@@ -51,6 +51,25 @@ def test_ties_go_to_the_even_integer(cuda_lib, M, K, dtype, kind):
     assert torch.equal(q.double(), quotient.round())
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("K, pad", [(2048, 0), (2048, 1), (2056, 0), (70000, 0)])
+def test_every_mantissa_under_every_largest_value(cuda_lib, K, pad, dtype):
+    """Row b: all multiples of a step up to b steps, b from half to all of what the type's mantissa holds; then, under the
+    same largest value, a half, a quarter ... of them."""
+    top = 2048 if dtype == torch.float16 else 256
+    b = torch.arange(top // 2, top, device="cuda")
+    step = torch.arange(K, device="cuda") % top
+    x = torch.empty(len(b), K + pad, dtype=dtype, device="cuda")[:, :K]
+    x.copy_(torch.where(step[None, :] <= b[:, None], step, b[:, None] - step))
+    q, s = torch.empty(len(b), K, dtype=torch.int8, device="cuda"), torch.empty(len(b), device="cuda")
+    for fraction in range(8):
+        if fraction:
+            x.mul_(0.5)
+            x[:, -1] = b.to(dtype)
+        api.RowQuantizer()(api.RowQuantizeArguments(x=x, q=q, scale=s))
+        assert torch.equal(q.double(), _quotient(x.double()).round())
+
+
 @pytest.mark.parametrize("dtype, kind", [(torch.float16, "normal"), (torch.bfloat16, "normal"), (torch.float16, "grid"),
                                          (torch.bfloat16, "grid"), (torch.bfloat16, "tiny grid")])
 @pytest.mark.parametrize("M, K", TIE_SHAPES)
