@@ -378,7 +378,7 @@ mgv_status mgv_rmsnorm_quantize(const mgv_rmsnorm_args *args, mgv_stream_t s);
  *   v[m][n] = x_scale[m] * weight_scale[n] * sum_k x[m][k] * weights[n][k] + bias[n]
  *   out[m][n] = round(act(v[m][n]))
  * The sum is exact (32-bit integers), so results do not depend on how the work is divided; the
- * epilogue computes in fp32 and rounds once.  weights are NOT preprocessed: the int8 matrix as
+ * epilogue computes (sum * weight_scale) * x_scale + bias in fp32 and rounds once.  weights are NOT preprocessed: the int8 matrix as
  * mgv_preprocess_weights takes it with MGV_LAYOUT_COLUMN_MAJOR, K contiguous for each feature.
  * A layer that also decodes through mgv_gemv keeps both forms (the GEMV's interleave follows the
  * reference and is not one the tensor cores' 8-bit operands can be copied from).  Waits inside

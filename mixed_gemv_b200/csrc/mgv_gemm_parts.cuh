@@ -241,19 +241,21 @@ __device__ __forceinline__ Feature load_feature(const GemmI8Params &p, int n) {
 }
 
 // Sums of C neighbouring activation rows from m on for the lane's feature -- `rows` of them exist --
-// scaled, activated and stored.  Lanes 2i and 2i + 1 swap half of their values, so that the even
-// lane holds both features of the even rows and the odd lane both of the odd rows: one 32-bit store for two
-// features, or gate and up together.  All 32 lanes call it; x_scale is 16-byte aligned.
+// scaled, activated and stored.  The sum takes the feature's scale first: the two scales' product may be beyond fp32
+// (infinite, or short of bits) where the value is not; a sum times a weight's scale below 2^96 is not, and a sum of zero
+// stays zero.  Lanes 2i and 2i + 1 swap half of their values, so that the even lane holds both features of the even rows
+// and the odd lane both of the odd rows: one 32-bit store for two features, or gate and up together.  All 32 lanes call it;
+// x_scale is 16-byte aligned.
 template <int ACT, bool BF16, int C>
 __device__ __forceinline__ void finish(const GemmI8Params &p, const Feature &f, int m, int rows, const int (&v)[C], const float *x_scale) {
   float y[C];
 #pragma unroll
   for (int i = 0; i < C; i += 4) {
     const float4 s = *reinterpret_cast<const float4 *>(x_scale + i);
-    y[i] = fmaf(float(v[i]), f.scale * s.x, f.bias);
-    y[i + 1] = fmaf(float(v[i + 1]), f.scale * s.y, f.bias);
-    y[i + 2] = fmaf(float(v[i + 2]), f.scale * s.z, f.bias);
-    y[i + 3] = fmaf(float(v[i + 3]), f.scale * s.w, f.bias);
+    y[i] = fmaf(float(v[i]) * f.scale, s.x, f.bias);
+    y[i + 1] = fmaf(float(v[i + 1]) * f.scale, s.y, f.bias);
+    y[i + 2] = fmaf(float(v[i + 2]) * f.scale, s.z, f.bias);
+    y[i + 3] = fmaf(float(v[i + 3]) * f.scale, s.w, f.bias);
   }
   if (ACT == kActRelu || ACT == kActSilu) {
 #pragma unroll

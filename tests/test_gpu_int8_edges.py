@@ -1,9 +1,12 @@
-"""GPU tests of the 8-bit activation path at its edges: ties of the quantisation, long rows."""
+"""GPU tests of the 8-bit activation path at its edges: ties of the quantisation, long rows, scales at the ends of their range.
+
+Tolerances count roundings.  U = 2^-24 is half a step of fp32 relative to the value.
+"""
 import pytest
 import torch
 
-from mixed_gemv_b200 import api
-from tests.test_gpu_int8_path import U, _check_quantised, _gen, _norm_reference
+from mixed_gemv_b200 import _lib, api
+from tests.test_gpu_int8_path import ACTS, U, Product, _check_quantised, _gen, _norm_reference
 
 pytestmark = pytest.mark.gpu
 
@@ -100,3 +103,23 @@ def test_norm_of_a_long_row_of_one_value(cuda_lib, K):
     api.RmsNormQuantizer()(api.RmsNormQuantizeArguments(x=x, weight=w, q=q, scale=s, eps=0.0))
     # the scale as in test_rmsnorm of the shorter rows
     _check_quantised(q, s, _norm_reference(x, None, w, 0.0)[1], 4 * U, 154 * U)
+
+
+# ---- the product's epilogue at the ends of its range --------------------------------------------
+
+PAIR, BLOCK = _lib.GEMM_HINT_PAIR, _lib.GEMM_HINT_BLOCK
+
+
+@pytest.mark.parametrize("hints", [BLOCK, PAIR])
+@pytest.mark.parametrize("act", list(ACTS))
+def test_scales_whose_product_is_beyond_fp32(cuda_lib, act, hints):
+    """Sums times their scales are numbers, the two scales' product is not: infinite, subnormal or zero."""
+    M, N, K = 40, 64, 96
+    for xs, ws, bias in ((2.0 ** 120, 2.0 ** 10, True), (2.0 ** -130, 2.0 ** -14, False), (2.0 ** -140, 2.0 ** -14, False),
+                         (2.0 ** -110, 2.0 ** -30, False), (2.0 ** -12, 2.0 ** -130, False)):
+        p = Product(M, N, K, torch.bfloat16, act=act, bias=bias, seed=3)
+        p.xs.copy_(xs * (1 + torch.arange(M, device="cuda") / 64))
+        p.ws.copy_(ws * (1 + torch.arange(N, device="cuda") / 128))
+        if xs > 1:
+            p.w.zero_()  # sums of zero: the bias alone is left
+        p.run(hints=hints).check()
