@@ -216,8 +216,18 @@ __device__ __forceinline__ float load_as_float(const void *p, int64_t i, int dty
   return static_cast<const float *>(p)[i];
 }
 
-// v / (1 + exp(-v)); exp and the quotient err by a few steps of fp32, far below the 16-bit output
-__device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
+// v / (1 + exp(-v)) = v m^2 / (1 + h^2) with h = exp(-|v| / 2) and m = h below zero, 1 above: neither the exponential nor the
+// denominator, which is in 1..2, leaves fp32's normal numbers before the result does, so a bf16 gate far below zero keeps its
+// value (v / (1 + exp(-v)) itself is 0 from -88 on).  The argument of 2^x errs by |v| steps of 2^-24, the square by twice as much:
+// 2^-16 of the value at -100, far below the 16-bit output.  The approximate instructions on normal numbers need no care
+// around them: 4096 x 8192 x 1024 gated 48.0 us, with __expf and __fdividef 57.0, with v / (1 + __expf(-v)) 51.7.
+__device__ __forceinline__ float silu(float v) {
+  float h, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(h) : "f"(fabsf(v) * -0.72134752f));  // log2(e) / 2
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(h, h, 1.0f)));
+  const float m = v > 0.0f ? 1.0f : h;
+  return v * m * (m * r);
+}
 
 template <bool BF16>
 __device__ __forceinline__ uint16_t round_out(float v) {

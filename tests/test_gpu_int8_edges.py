@@ -1,4 +1,5 @@
-"""GPU tests of the 8-bit activation path at its edges: ties of the quantisation, long rows, scales at the ends of their range.
+"""GPU tests of the 8-bit activation path at its edges: ties of the quantisation, long rows, scales and gates at the ends
+of their range.
 
 Tolerances count roundings.  U = 2^-24 is half a step of fp32 relative to the value.
 """
@@ -123,3 +124,25 @@ def test_scales_whose_product_is_beyond_fp32(cuda_lib, act, hints):
         if xs > 1:
             p.w.zero_()  # sums of zero: the bias alone is left
         p.run(hints=hints).check()
+
+
+@pytest.mark.parametrize("hints", [BLOCK, PAIR])
+@pytest.mark.parametrize("act", ["silu", "gated"])
+def test_gates_far_below_zero(cuda_lib, act, hints):
+    """v / (1 + exp(-v)) for v from -80 to -110: bf16 holds it down to -92 as a normal number, and beyond as a subnormal one."""
+    M, N, K = 40, 480, 32
+    p = Product(M, N, K, torch.bfloat16, act=act, bias=True, seed=4)
+    p.x.zero_()
+    gates = -80 - torch.arange(N, device="cuda") / 16
+    p.bias.copy_(gates)
+    if act == "gated":
+        p.bias[1::2] = 3
+    p.run(hints=hints)
+    v = p.bias.double()
+    want = v / (1 + torch.exp(-v))
+    if act == "gated":
+        want = want[0::2] * 3
+    # exp(v): the argument times log2(e) errs by 2^-23 of |v| * 1.44 in its exponent, 2^-16 of the value at 110; ten more roundings
+    # of fp32 and one to bf16 (2^-8), whose subnormal step is 2^-133, and fp32's below 2^-126, times up to 3, 2^-149
+    off = (p.out.double() - want).abs() - ((2.0 ** -8 + 2.0 ** -15) * want.abs() + 2.0 ** -134 + 2.0 ** -147)
+    assert float(off.max()) <= 0, p.out[0, off.argmax().item() % p.out.shape[1]]
