@@ -81,6 +81,9 @@ __global__ void __launch_bounds__(kGemmThreads, kGemmBlocksPerSm) gemm_i8_block_
     for (int i = max(0, issued - p.stages); i < issued; ++i)
       if (!bar_wait(smem_u32(&sh.full[i % p.stages]), (i / p.stages) & 1, p.err)) break;
   } else if (warp == 1) {
+    // its wait for the first slot is limited, and the slot's activations are asked for behind the wait above: what the
+    // previous kernel still takes is not to count
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     int slot = 0;
     uint32_t phase = 0;
     bool ok = true;

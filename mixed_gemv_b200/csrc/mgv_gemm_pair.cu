@@ -105,6 +105,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_pair_kernel(const __g
       for (uint32_t i = issued > uint32_t(p.stages) ? issued - p.stages : 0; i < issued; ++i)
         if (!bar_wait(smem_u32(&sh.full[i % p.stages]), (i / p.stages) & 1, p.err)) break;
   } else if (warp == 1 && rank == 0) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // its limited waits count from the previous kernel's end
     const bool one = elect_one();
     int slot = 0;
     uint32_t phase = 0, turn = 0;

@@ -1,5 +1,5 @@
 """GPU tests of the 8-bit activation path at its edges: ties of the quantisation, long rows, scales and gates at the ends
-of their range.
+of their range, slow predecessors.
 
 Tolerances count roundings.  U = 2^-24 is half a step of fp32 relative to the value.
 """
@@ -146,3 +146,39 @@ def test_gates_far_below_zero(cuda_lib, act, hints):
     # of fp32 and one to bf16 (2^-8), whose subnormal step is 2^-133, and fp32's below 2^-126, times up to 3, 2^-149
     off = (p.out.double() - want).abs() - ((2.0 ** -8 + 2.0 ** -15) * want.abs() + 2.0 ** -134 + 2.0 ** -147)
     assert float(off.max()) <= 0, p.out[0, off.argmax().item() % p.out.shape[1]]
+
+
+# ---- a predecessor that takes long --------------------------------------------------------------
+
+@pytest.fixture(scope="module")
+def slow_predecessor(tmp_path_factory):
+    """Enqueues a kernel of that many seconds which lets its dependents start at once."""
+    import ctypes as C
+    import os
+    import subprocess
+    from mixed_gemv_b200 import build
+    out = str(tmp_path_factory.mktemp("slow") / "slow_predecessor.so")
+    src = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "slow_predecessor.cu")
+    subprocess.run([build._nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", "-shared", "-Xcompiler", "-fPIC", src,
+                    "-o", out], check=True, capture_output=True, timeout=300)
+    fn = C.CDLL(out).slow_predecessor
+    fn.argtypes = [C.c_ulonglong, C.c_void_p]
+    return lambda seconds: fn(int(seconds * 1e9), torch.cuda.current_stream().cuda_stream)
+
+
+@pytest.mark.parametrize("hints", [BLOCK, PAIR, BLOCK | _lib.gemm_hint_split(4) | _lib.gemm_hint_rows(32),
+                                   PAIR | _lib.gemm_hint_split(2) | _lib.gemm_hint_rows(64)])
+def test_the_limit_of_the_waits_does_not_count_the_predecessor(cuda_lib, slow_predecessor, hints):
+    """The kernels' waits give up after a second; a dependent launch that starts early waits for its predecessor first."""
+    p = Product(70, 600, 1100, bias=True, seed=9)
+    op = api.GemmI8Adaptor()
+    op.initialize(p.arguments(_lib.FLAG_PDL, hints))
+    op.run()
+    torch.cuda.synchronize()
+    p.out.fill_(1234.0)
+    torch.cuda.synchronize()
+    assert slow_predecessor(1.5) == 0
+    op.run()
+    torch.cuda.synchronize()
+    assert api.device_error_state() == 0
+    p.check()
