@@ -410,7 +410,7 @@ typedef struct mgv_gemm_i8_args {
  * kernel or tiling; they exist so that tests and tuning runs can reach each path on any shape.
  * Bits 8..12: rows of x in a tile, in units of 16 (rounded up to what the kernel takes; 0:
  * the library chooses the tiling).  Bits 0..2, with those: blocks (1..8) or pairs of blocks (1, 2, 4)
- * that share a tile's K range, less 1; fewer where K is short. */
+ * that share a tile's K range, less 1; fewer where K is short.  Other bits are refused. */
 enum {
   MGV_GEMM_HINT_BLOCK = 8,  /* the kernel of single blocks (small batches)                        */
   MGV_GEMM_HINT_PAIR = 16   /* the kernel of block pairs (prompts)                                */

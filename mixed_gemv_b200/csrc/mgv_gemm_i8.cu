@@ -190,6 +190,8 @@ static mgv_status check_args(const mgv_gemm_i8_args *a) {
   if (act & (act - 1)) return fail(MGV_STATUS_INVALID_ARGUMENT, "gemm_i8: one activation at most (flags %d)", a->flags);
   const bool gated = act == MGV_FLAG_GATED_SILU;
   if (gated && a->N % 2) return fail(MGV_STATUS_INVALID_ARGUMENT, "gemm_i8: a gated layer needs an even N (%d)", a->N);
+  constexpr int hints = 7 | MGV_GEMM_HINT_BLOCK | MGV_GEMM_HINT_PAIR | 31 << 8;
+  if (a->hints & ~hints) return fail(MGV_STATUS_INVALID_ARGUMENT, "gemm_i8: unknown bits in hints %d", a->hints);
   if (a->reserved) return fail(MGV_STATUS_INVALID_ARGUMENT, "gemm_i8: reserved must be 0");
   if (a->M == 0) return MGV_STATUS_OK;
   if (!a->x || !a->weights || !a->x_scale || !a->weight_scale || !a->out) return fail(MGV_STATUS_INVALID_ARGUMENT, "gemm_i8: null operand");
