@@ -3,6 +3,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
 #include <cmath>
 #include <type_traits>
@@ -167,7 +168,7 @@ struct RowStats {
 };
 // The fp32 statistics serve: squares, products and their quotients are numbers well inside fp32.
 template <bool NORM>
-__device__ __forceinline__ bool row_is_tame(const RowParams &p, const RowStats &s, float mean) {
+__device__ __forceinline__ bool row_is_tame(const RowStats &s, float mean) {
   const bool sum_ok = !NORM || (mean >= 1e-30f && mean <= FLT_MAX);
   return sum_ok && (s.top == 0 || (s.top >= __float_as_uint(1e-30f) && s.top < 0x7f800000u));
 }
@@ -354,7 +355,7 @@ __global__ void __launch_bounds__(WARP_ROW ? 128 : 1024, WARP_ROW ? 6 : 1) rows_
     }
     s = WARP_ROW ? warp_stats(s) : block_stats(s, stats[turn]);
     const float mean = s.ss / float(p.K) + p.eps;
-    const bool tame = row_is_tame<NORM>(p, s, mean);
+    const bool tame = row_is_tame<NORM>(s, mean);
     if (!tame) {
       if (t == 0) p.scale[m] = kLeft;
       left = true;
@@ -455,7 +456,7 @@ __global__ void __launch_bounds__(kLongThreads, 3) long_rows_kernel(const __grid
   if (NORM) fold();
   s = block_stats(s, stats);
   const float mean = s.ss / float(p.K) + p.eps;
-  if (!row_is_tame<NORM>(p, s, mean)) {
+  if (!row_is_tame<NORM>(s, mean)) {
     row_in_double<T, NORM, false>(p, m, threadIdx.x, kLongThreads, buf);
     return;
   }
@@ -568,11 +569,13 @@ static bool aligned_rows(const void *p, int64_t ld, int64_t elem, int64_t rows, 
 }
 
 static int sm_count() {
-  static int count[64];
+  static std::atomic<int> known[64];  // calls may come from several threads
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  if (!count[dev] && cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) count[dev] = 0;
-  return count[dev] ? count[dev] : 148;
+  int count = known[dev].load(std::memory_order_relaxed);
+  if (!count && cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess)
+    known[dev].store(count, std::memory_order_relaxed);
+  return count > 0 ? count : 148;
 }
 
 template <typename T, bool NORM>

@@ -182,3 +182,34 @@ def test_the_limit_of_the_waits_does_not_count_the_predecessor(cuda_lib, slow_pr
     torch.cuda.synchronize()
     assert api.device_error_state() == 0
     p.check()
+
+
+THREADS = """
+import threading
+import torch
+from mixed_gemv_b200 import api
+x = [torch.randn(700, 512 + 8 * i, dtype=torch.float32, device="cuda").half() for i in range(8)]
+q = [torch.empty(t.shape, dtype=torch.int8, device="cuda") for t in x]
+s = [torch.empty(700, device="cuda") for t in x]
+torch.cuda.synchronize()
+start = threading.Barrier(8)
+def one(i):
+    start.wait()
+    api.RowQuantizer()(api.RowQuantizeArguments(x=x[i], q=q[i], scale=s[i]), torch.cuda.Stream())
+threads = [threading.Thread(target=one, args=(i,)) for i in range(8)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+torch.cuda.synchronize()
+for a, b, c in zip(x, q, s):
+    y = a.double()
+    assert torch.equal(b.double(), (y * 127 / y.abs().amax(dim=1, keepdim=True)).round())
+print("threads agree")
+"""
+
+
+def test_first_calls_from_several_threads(cuda_lib):
+    import subprocess
+    import sys
+    from tests.conftest import ROOT
+    r = subprocess.run([sys.executable, "-c", THREADS], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "threads agree" in r.stdout, r.stderr[-2000:]
