@@ -1,5 +1,5 @@
 """GPU tests of the 8-bit activation path at its edges: ties of the quantisation, long rows, scales and gates at the ends
-of their range, slow predecessors.
+of their range, clusters of every size, slow predecessors.
 
 Tolerances count roundings.  U = 2^-24 is half a step of fp32 relative to the value.
 """
@@ -146,6 +146,33 @@ def test_gates_far_below_zero(cuda_lib, act, hints):
     # of fp32 and one to bf16 (2^-8), whose subnormal step is 2^-133, and fp32's below 2^-126, times up to 3, 2^-149
     off = (p.out.double() - want).abs() - ((2.0 ** -8 + 2.0 ** -15) * want.abs() + 2.0 ** -134 + 2.0 ** -147)
     assert float(off.max()) <= 0, p.out[0, off.argmax().item() % p.out.shape[1]]
+
+
+# ---- clusters of every size ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("hints", [BLOCK | _lib.gemm_hint_split(s) | _lib.gemm_hint_rows(r) for s in range(1, 9) for r in (16, 32, 96, 256)] +
+                         [PAIR | _lib.gemm_hint_split(s) | _lib.gemm_hint_rows(r) for s in (1, 2, 4) for r in (32, 256)])
+@pytest.mark.parametrize("M, N, K, act", [(1, 100, 1090, "none"), (77, 300, 1300, "silu"), (263, 642, 2049, "gated")])
+def test_every_cluster_size_writes_every_element(cuda_lib, M, N, K, act, hints):
+    p = Product(M, N, K, act=act, bias=True, seed=6, ldd=(N // 2 if act == "gated" else N) + 3)
+    p.run().check()
+    want = p.out.clone()
+    p.out.fill_(1234.0)
+    p.run(hints=hints)
+    assert torch.equal(p.out, want)
+    assert api.device_error_state() == 0
+    p.check_surroundings()
+
+
+@pytest.mark.parametrize("M", [4, 300])
+def test_rows_beside_one_without_a_scale_are_written(cuda_lib, M):
+    p = Product(M, 260, 320, bias=True, seed=2).run()
+    want = p.out.clone()
+    p.xs[1] = float("nan")
+    p.out.fill_(1234.0)
+    p.run()
+    keep = [i for i in range(M) if i != 1]
+    assert bool(p.out[1].isnan().all()) and torch.equal(p.out[keep], want[keep])
 
 
 # ---- a predecessor that takes long --------------------------------------------------------------
