@@ -333,9 +333,9 @@ mgv_status mgv_gemv_launch_info(const mgv_gemv_args *args, mgv_launch_info *info
  * M = 0 (no rows) is a valid call that launches nothing.  MGV_FLAG_PDL works as in the GEMV: the
  * kernel may start while its predecessor on the stream drains, and touches only norm weights,
  * layer weights, their scales and bias before that predecessor has completed.  Those must not be
- * written by the predecessor, nor by a kernel before it where the predecessor is a GEMV launched
- * with MGV_FLAG_PDL (which lets its dependents start before its own predecessor has ended; the
- * kernels here do not).  Outputs must not overlap inputs, except as stated. */
+ * written by the predecessor, nor by a kernel before it where the predecessor lets its dependents
+ * start before its own predecessor has ended: mgv_gemv and mgv_wait_reduce_partials with
+ * MGV_FLAG_PDL do, and so may a kernel of your own; the kernels here do not.  Outputs must not overlap inputs, except as stated. */
 
 typedef enum mgv_dtype { MGV_DTYPE_F16 = 0, MGV_DTYPE_BF16 = 1, MGV_DTYPE_F32 = 2 } mgv_dtype;
 

@@ -57,8 +57,8 @@ __global__ void __launch_bounds__(kGemmThreads, kGemmBlocksPerSm) gemm_i8_block_
   if (p.split > 1 && p.sums_off) cluster_arrive<true>();  // this block can be sent to: its barriers are set up
 
   if (warp == 0) {
-    // A dependent kernel may start only now: behind the wait, so that no kernel runs beside any but its direct
-    // predecessor, and behind the allocation of tensor memory, of which it may hold some while it waits for this one.
+    // A dependent kernel may start only now: behind the wait, so that it runs beside no kernel but this one, and
+    // behind the allocation of tensor memory, of which it may hold some while it waits for this one.
     asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;\n\tfence.proxy.async.global;" ::: "memory");
     if (one) {
       for (int i = 0; i < ahead; ++i)

@@ -12,9 +12,10 @@
 
 namespace mgv {
 
-// Waits for the stream's previous kernel (dependent launches), and only then lets the next one start: so no
-// kernel runs beside any but its direct predecessor, and what it touches before its own wait only has to be
-// older than that.
+// Waits for the stream's previous kernel (dependent launches), and only then lets the next one start: so what
+// follows these kernels runs beside its direct predecessor only, and what it touches before its own wait only
+// has to be older than that.  (Behind a kernel that lets its dependents start before its own wait, as the GEMV and the
+// wait for partials do, it has to be older than what that one waits for too.)
 __device__ __forceinline__ void wait_for_previous() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
