@@ -251,7 +251,7 @@ static uint32_t instruction(int rows, int columns) { return 2u << 4 | 1u << 7 | 
 // The estimate that tilings are compared by, in cycles.  Measured on B200 (4096-deep reductions, 1.9 GHz): an
 // SM alone takes in 96 bytes a cycle from L2, all SMs together 7500 as single blocks and 9400 as pairs; a slice of
 // 128 K keeps the issuing warp for 330 cycles at least and the matrix unit for the time of its four
-// instructions; HBM delivers 3260 bytes a cycle but for the start and end of a block's row of slices; 16
+// instructions (taken as half a cycle a column each, 40 at least; measured 127 at 256 columns); HBM delivers 3260 bytes a cycle but for the start and end of a block's row of slices; 16
 // columns of an epilogue take 320 cycles; a split tile's exchange takes 1500 and, a column, 30 and
 // 5 for each part beside the next call's start.
 // (Of 20 shapes from 1 x 4096 x 4096 to 4096 x 4096 x 4096 -- rows x features x K -- the choice was within 8 % of the best

@@ -25,9 +25,9 @@ __device__ __forceinline__ TileAt tile_at(const GemmI8Params &p, uint32_t item) 
 // matrix instructions for both.  Two accumulators in tensor memory: the epilogue of a tile runs
 // beside the next tile's products.  Tiles too few for the GPU are shared by the p.split pairs of a cluster.  Where the last round of tiles would leave half of the pairs or more without
 // one, its tiles are halved: 2048 x 8192 features at 256 rows are 3.46 tiles to a pair, in 3.5 rounds instead of 4.
-// Bound by the matrix unit (508 cycles for a slice of a 256-row tile; its instructions take 512) and, over more than a
+// Bound by the matrix unit (508 cycles for a slice of a 256-row tile: four instructions of 127) and, over more than a
 // few milliseconds, by the power limit: B200, 4096 x 4096 x 4096 43.9 us (3.13 POP/s at 1.9 GHz), 4096 x 57344 x 8192 gated
-// 1.30 ms (2.96 POP/s at 1.2 - 1.3 GHz); 256 x 4096 x 11008 as 32 tiles of two pairs each 15.2 us, one pair each 17.4.
+// 1.28 ms (3.00 POP/s at 1.2 - 1.3 GHz); 256 x 4096 x 11008 as 32 tiles of two pairs each 15.2 us, one pair each 17.4.
 template <int ACT, bool BF16>
 __global__ void __launch_bounds__(kGemmThreads, 1) gemm_i8_pair_kernel(const __grid_constant__ GemmI8Params p) {
   extern __shared__ uint8_t dynamic[];

@@ -214,8 +214,8 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 // an inv that is not below 127 / top.  Rows whose top has 127 in its mantissa (one in 127 of fp16 rows; of bf16 rows their
 // inv is exact) take two terms.  (Tried on every pair of mantissas.)
 //
-// B200, 4096 x 8192 bf16: quantisation 16.9 us in one term, 18.2 in two (19.1 with one value an instruction); the norm 39.1
-// in two terms.
+// B200, 4096 x 8192 bf16: quantisation 16.8 us in one term, 18.3 in two (19.1 with one value an instruction); the norm with
+// residual, in two, 38.7 (40.6).
 struct RowFactors {
   float scale, inv, rest;  // inv + rest has 40 bits and more (28 for a top near fp32's largest, where rest is subnormal)
   bool two;
@@ -268,7 +268,8 @@ constexpr float kLeft = -1.0f;
 // r max|h w| / 127 and q = h w 127 / max|h w|, in which r does not occur.  The sum of squares, the
 // largest value and the scale are fp32.  A block takes a row (a warp, for short rows) with NV pieces of V
 // values to a thread, then the next one; the norm's weights stay in registers over its rows where there is room.
-// Bound by HBM: B200, 4096 x 8192 bf16 with residual 37.8 us (6.2 TB/s, 0.95 of the copy bandwidth), without norm 16.5 us.
+// Bound by HBM: B200, 4096 x 8192 bf16 with residual 38.7 us (6.1 TB/s, 0.93 of the copy bandwidth), without norm 16.8 us.
+// Two forms spill, at the 64 registers of a 1024-thread block: the norm with eight pieces a thread (44 bytes) and the norm value by value (16).
 template <typename T, bool NORM, int V, int NV, bool WARP_ROW>
 __global__ void __launch_bounds__(WARP_ROW ? 128 : 1024, WARP_ROW ? 6 : 1) rows_kernel(const __grid_constant__ RowParams p) {
   constexpr bool kKeepWeight = NV <= 2 || (V == 1 && NV == 8);
@@ -592,7 +593,7 @@ static mgv_status quantise(const RowParams &p, int flags, cudaStream_t s) {
       return launch_rows(rows_kernel<T, NORM, 8, 4, true>, std::min<int64_t>((p.M + 3) / 4, int64_t(sms) * 16), 128, flags, s, p);
     // few rows: as many threads as a row has pieces, for the shortest chain of loads; many rows: more pieces a thread and
     // smaller blocks, so that several of an SM are at different points of their rows (norm of 4096 x 8192 with residual
-    // 42.9 us with four pieces, 37.8 with two and the next row on its way; quantisation 22.9 us with two, 16.5 with four)
+    // 43.2 us with four pieces, 38.7 with two and the next row on its way; quantisation 18.9 us with two, 16.8 with four)
     int nv = 1;
     while (nv < 8 && pieces > 1024 * nv) nv *= 2;
     if (p.M > few) nv = std::max(nv, NORM ? 2 : 4);
@@ -606,7 +607,7 @@ static mgv_status quantise(const RowParams &p, int flags, cudaStream_t s) {
     }
   }
   // Value by value: in registers where rows are short or few, else in two passes (the norm of 1000 rows of 5001:
-  // 16.6 us against 22.5).
+  // 9.7 us against 12.3, with residual 13.0 against 16.4).
   if (p.K <= 2048 || (p.K <= 8192 && p.M <= few)) {
     const int threads = ((p.K + 7) / 8 + 31) / 32 * 32;
     return launch_rows(rows_kernel<T, NORM, 1, 8, false>, std::min<int64_t>(p.M, int64_t(sms) * (2048 / threads)), threads, flags, s, p);
